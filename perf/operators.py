@@ -353,8 +353,9 @@ def _plain_prefix(s):
 
 def _plain_verify(s):
     """Draft i of a sequence stands if u_i q_i(token) < p_i(token) and all before it stand. The token after the a
-    that stand is drawn from max(p_a - q_a, 0), or from p_a where no draft was refused, at uniform number u_a: the
-    first v whose running sum of the weights, in units of 2^-40, is above that share of their sum."""
+    that stand is drawn from max(p_a - q_a, 0), or from p_a where no draft was refused, at the row's last uniform
+    number (which no draft was tested against): the first v whose running sum of the weights, in units of 2^-40, is
+    above that share of their sum."""
     target, draft, tokens, u = s["target"], s["draft"], s["tokens"], s["uniforms"]
     batch, most, vocab = draft.shape
     count = s["counts"].long() if s["counts"] is not None else torch.full((batch,), most, device="cuda")
@@ -373,7 +374,7 @@ def _plain_verify(s):
     units = torch.where(units.sum(dim=-1, keepdim=True) == 0, whole, units)
     running = units.cumsum(dim=-1)
     total = running[:, -1]
-    share = (u[b, accepted] * 2.0 ** 24).to(torch.int64)
+    share = (u[:, most] * 2.0 ** 24).to(torch.int64)
     goal = share * (total >> 24) + ((share * (total & (2 ** 24 - 1))) >> 24)
     follows = (running <= goal[:, None]).sum(dim=-1)
     at = torch.arange(most + 1, device="cuda")
@@ -462,7 +463,7 @@ def _exact_verify(s):
         units = torch.floor(w * 2.0 ** 40).long()
         if int(units.sum()) == 0:
             units = torch.floor(p.clamp(0, 1) * 2.0 ** 40).long()
-        goal = int(u[b][a] * 2 ** 24) * int(units.sum()) >> 24
+        goal = int(u[b][most] * 2 ** 24) * int(units.sum()) >> 24
         follows = int(torch.searchsorted(units.cumsum(0), goal, right=True))
         out.append(tokens[b][:a] + [follows] + [-1] * (most - a))
         accepted.append(a)
