@@ -375,6 +375,128 @@ QI4_API int qi4_bf16_gemv_argmax_ws(const void* weight, const void* x, int64_t M
  * Returns QI4_ERR_SHAPE unless 1 <= B < 2^31, 1 <= V < 2^32, ld >= V. */
 QI4_API int qi4_bf16_argmax_rows(const void* logits, int64_t B, int64_t V, int64_t ld, int64_t* out, void* stream);
 
+/*
+ * Paged KV cache and ragged batches. One layer's cache is a pool of `pages`
+ * pages, each holding page_size consecutive positions of one sequence:
+ *   K of (page, head, slot) at k + page * page_stride + head * head_stride +
+ *   slot * slot_stride (elements; V alike), head_dim contiguous elements.
+ * Position p of sequence b lies in page block_table[b * table_stride +
+ * p / page_size], slot p % page_size. page_size is a power of two from 8 to
+ * 1024; k and v are 16-byte aligned, the strides multiples of 8 elements, so
+ * [pages, heads, slots, dim] and [pages, slots, heads, dim] pools both fit.
+ *
+ * A batch of B sequences brings T new tokens, the rows of [T, heads, dim]
+ * tensors: sequence b owns rows cu_tokens[b] .. cu_tokens[b + 1] - 1 (device,
+ * int32, B + 1 entries, ascending; a sequence may have none), or T / B rows
+ * each when cu_tokens is NULL.
+ *
+ * No device array can make a kernel touch memory outside the tensors: token
+ * ranges are clipped to T, positions beyond the table and pages outside the
+ * pool are not written (and read as zeros), and qi4_device_status reports
+ * QI4_DEVICE_CACHE_FULL (position beyond the block table), QI4_DEVICE_BAD_PAGE,
+ * QI4_DEVICE_BAD_POSITION (no such row of cos / sin; the nearest is used) and
+ * QI4_DEVICE_BAD_TOKEN (a drafted token outside the vocabulary).
+ */
+#define QI4_DEVICE_BAD_PAGE 4
+#define QI4_DEVICE_BAD_POSITION 8
+#define QI4_DEVICE_BAD_TOKEN 16
+typedef struct qi4_paged_kv {
+  void* k;
+  void* v;
+  const int32_t* block_table; /* [B, table_width], rows table_stride apart */
+  int64_t table_stride;
+  int64_t page_stride, head_stride, slot_stride; /* elements, K and V alike */
+  int32_t dtype;                                 /* QI4_DTYPE_BF16 or QI4_DTYPE_F16 */
+  int32_t pages, page_size, kv_heads, head_dim, table_width;
+} qi4_paged_kv;
+
+/*
+ * Rotary positions on the new queries and keys, and the append of the new keys
+ * and values: token i of sequence b is at position p = lengths[b] + i
+ * (lengths: keys cached before this call), and
+ *   q_out[t, h] = rotate(q[t, h]),  K page slot of p = rotate(k[t, h]),
+ *   V page slot of p = v[t, h]
+ * where rotate turns the first rot_dim dimensions by row positions[t] (or p
+ * when positions is NULL) of cos / sin (FP32, [rope_rows, rot_dim / 2],
+ * contiguous): pairs (m, m + rot_dim / 2), or (2m, 2m + 1) when interleaved:
+ *   x' = x c - y s,  y' = y c + x s   (FP32, one rounding to the cache's type).
+ * q, k, v and q_out have the cache's type, head_dim contiguous, and token /
+ * head strides that are multiples of 8 elements; q_out may be q. head_dim and
+ * rot_dim are multiples of 16; rot_dim = 0 appends without rotation; Hq = 0
+ * has no queries. lengths is not modified. Replaces, for a paged cache, the
+ * rotation and the cache growth of reference src/qwen_int4/model.py:74-88.
+ */
+QI4_API int qi4_rope_paged_append(const qi4_paged_kv* kv, const void* q, int64_t q_token_stride,
+                                  int64_t q_head_stride, const void* k, int64_t k_token_stride,
+                                  int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                                  int64_t v_head_stride, void* q_out, int64_t out_token_stride,
+                                  int64_t out_head_stride, int64_t T, int64_t B, int64_t Hq,
+                                  const int32_t* cu_tokens, const int32_t* lengths, const int32_t* positions,
+                                  const float* cos, const float* sin, int64_t rope_rows, int rot_dim,
+                                  int interleaved, void* stream);
+
+/*
+ * Attention of the new tokens over their sequences' pages:
+ *   out[t, h] = softmax(scale q[t, h] . K[j]) V[j] over the keys j that the
+ *   token sees of KV head h / (Hq / kv_heads)
+ * lengths[b] counts sequence b's keys, its new tokens' among them (they are
+ * appended before). causal: token i of n sees keys 0 .. lengths[b] - n + i;
+ * else all lengths[b]. A token that sees no key has a zero output. FP32
+ * scores, softmax and sums; the weights of the second product are carried to
+ * 16 bits or more where a tile has few rows, and rounded to the cache's type
+ * on the tcgen05 path (max_tokens * Hq / kv_heads large). What page slots
+ * beyond a length hold does not matter, NaN included. q as in
+ * qi4_rope_paged_append; out [T, Hq, head_dim] contiguous; head_dim 64 or 128.
+ * max_tokens: no sequence has more new tokens (0: not known); it only chooses
+ * the kernel. workspace: qi4_paged_attention_workspace bytes, 16-byte aligned,
+ * no initialisation needed, not shared by calls that may overlap; NULL: the
+ * library's scratch pool. Replaces, for a paged cache, reference
+ * src/qwen_int4/model.py:90-118.
+ */
+QI4_API int qi4_paged_attention(const qi4_paged_kv* kv, const void* q, int64_t q_token_stride,
+                                int64_t q_head_stride, void* out, int64_t T, int64_t B, int64_t Hq,
+                                const int32_t* cu_tokens, const int32_t* lengths, int64_t max_tokens, float scale,
+                                int causal, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The same for a batch whose sequences all begin with one prefix of
+ * prefix_length cached keys in the pages prefix_table[0 .. prefix_pages) of
+ * the same pool: every token sees all of the prefix and, causally, its own
+ * sequence's lengths[b] further keys (block_table covers these alone). The
+ * prefix is read once for the whole batch. The workspace is that of
+ * qi4_paged_attention_workspace with prefix = 1. No reference counterpart.
+ */
+QI4_API int qi4_shared_prefix_attention(const qi4_paged_kv* kv, const void* q, int64_t q_token_stride,
+                                        int64_t q_head_stride, void* out, int64_t T, int64_t B, int64_t Hq,
+                                        const int32_t* prefix_table, int64_t prefix_pages, int64_t prefix_length,
+                                        const int32_t* cu_tokens, const int32_t* lengths, int64_t max_tokens,
+                                        float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Workspace bytes of the two calls above on the current device (0 without one). */
+QI4_API size_t qi4_paged_attention_workspace(int64_t T, int64_t Hq, int head_dim, int prefix);
+
+/*
+ * Verification of drafted tokens (speculative decoding) from given uniform
+ * numbers in [0, 1). Draft i of sequence b stands while uniforms[b, i] *
+ * q_i(t_i) < p_i(t_i) (FP32) and all before it stand; after the a that stand,
+ * one token is drawn at uniforms[b, K] from max(p_a - q_a, 0), or from p_a when
+ * none of the sequence's draft_counts[b] (NULL: K) drafts was refused. Weights
+ * count in whole units of 2^-40, summed exactly: the drawn token is the first
+ * whose running sum exceeds floor(u 2^24) / 2^24 of the total; where
+ * max(p - q, 0) leaves nothing it is drawn from p_a, and is -1 where that has
+ * nothing either.
+ *   draft_tokens [B, K]; target_probs [B, K + 1, V] and draft_probs [B, K, V]
+ *   of `dtype` at the given strides (elements), V contiguous; draft_probs NULL:
+ *   drafts without a distribution (q = 1 at the token); uniforms [B, K + 1];
+ *   out_tokens [B, K + 1]: the standing drafts, the drawn token, then -1;
+ *   accepted [B]: a. K <= 4096, V <= 2^22. No reference counterpart.
+ */
+QI4_API int qi4_verify_draft(const int64_t* draft_tokens, const void* target_probs, int64_t target_batch_stride,
+                             int64_t target_pos_stride, const void* draft_probs, int64_t draft_batch_stride,
+                             int64_t draft_pos_stride, int dtype, const float* uniforms,
+                             const int32_t* draft_counts, int64_t B, int64_t K, int64_t V, int64_t* out_tokens,
+                             int32_t* accepted, void* stream);
+
 /* Tuning hook: forces the TMA/tensor-pipe GEMV launch shape for subsequent
  * calls made by the calling thread - output rows per CTA (16, 32, 64 or 128),
  * K-split factor (CTAs per cluster, 1..8) and warps per CTA (2, 4, 8, 16 or

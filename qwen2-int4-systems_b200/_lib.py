@@ -56,12 +56,20 @@ SIGNATURES = {
     "qi4_add_rmsnorm": [_p, _p, _i, _p, _p, _i64, _i64, ctypes.c_float, _p],
     "qi4_w4g64_linear_multi_norm": [_p, _i64, _i64, _i, _p, _p, _p, _p, _i, _p, _p, _p],
     "qi4_w4g64_gate_up_silu_norm": [_p, _i64, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _p],
+    "qi4_rope_paged_append": [_p, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _p,
+                              _p, _p, _p, _p, _i64, _i, _i, _p],
+    "qi4_paged_attention": [_p, _p, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _i64, ctypes.c_float, _i, _p, _sz, _p],
+    "qi4_shared_prefix_attention": [_p, _p, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _i64,
+                                    ctypes.c_float, _p, _sz, _p],
+    "qi4_paged_attention_workspace": [_i64, _i64, _i, _i],
+    "qi4_verify_draft": [_p, _p, _i64, _i64, _p, _i64, _i64, _i, _p, _p, _i64, _i64, _i64, _p, _p, _p],
     "qi4_last_error": [ctypes.c_char_p, _sz],
     "qi4_version": [],
 }
 
 # Return types other than the int status.
-RESTYPES = {"qi4_gqa_decode_attention_workspace": ctypes.c_size_t}
+RESTYPES = {"qi4_gqa_decode_attention_workspace": ctypes.c_size_t,
+            "qi4_paged_attention_workspace": ctypes.c_size_t}
 
 CHAIN_SWIGLU = 1
 ATTN_EARLY_CACHE_READ = 1
@@ -73,6 +81,18 @@ class RmsNormPrologue(ctypes.Structure):
     _fields_ = [
         ("h_in", ctypes.c_void_p), ("delta", ctypes.c_void_p), ("delta_dtype", ctypes.c_int32),
         ("eps", ctypes.c_float), ("weight", ctypes.c_void_p), ("h_out", ctypes.c_void_p),
+    ]
+
+
+class PagedKV(ctypes.Structure):
+    """``qi4_paged_kv`` of include/qi4_b200.h."""
+
+    _fields_ = [
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("block_table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64), ("page_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+        ("slot_stride", ctypes.c_int64), ("dtype", ctypes.c_int32), ("pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+        ("table_width", ctypes.c_int32),
     ]
 
 

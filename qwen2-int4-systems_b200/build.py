@@ -34,7 +34,7 @@ EXPORTS = [
     "qi4_w4g64_linear", "qi4_w4g64_linear_ex", "qi4_w4g64_dequant_f32",
     "qi4_w4_unpack", "qi4_w4g64_linear_f32_noalloc", "qi4_gemv_plan_override", "qi4_gemv_mma_plan_override", "qi4_gemm_tc_plan_override", "qi4_gemv_mma_plan", "qi4_w4g64_linear_multi", "qi4_w4g64_gate_up_silu", "qi4_device_status", "qi4_selftest_bounded_wait",
     "qi4_chain_create", "qi4_chain_run", "qi4_chain_info", "qi4_chain_destroy", "qi4_gqa_decode_attention", "qi4_bf16_gemv_argmax", "qi4_add_rmsnorm",
-    "qi4_w4g64_linear_multi_norm", "qi4_w4g64_gate_up_silu_norm", "qi4_gqa_decode_attention_workspace", "qi4_gqa_decode_attention_ex", "qi4_bf16_gemv_argmax_ws", "qi4_bf16_argmax_rows", "qi4_w4g64_gate_up_silu_scatter", "qi4_peer_flag_wait", "qi4_ipc_alloc", "qi4_ipc_open", "qi4_ipc_close", "qi4_ipc_free", "qi4_last_error", "qi4_version",
+    "qi4_w4g64_linear_multi_norm", "qi4_w4g64_gate_up_silu_norm", "qi4_gqa_decode_attention_workspace", "qi4_gqa_decode_attention_ex", "qi4_bf16_gemv_argmax_ws", "qi4_bf16_argmax_rows", "qi4_w4g64_gate_up_silu_scatter", "qi4_peer_flag_wait", "qi4_ipc_alloc", "qi4_ipc_open", "qi4_ipc_close", "qi4_ipc_free", "qi4_rope_paged_append", "qi4_paged_attention", "qi4_shared_prefix_attention", "qi4_paged_attention_workspace", "qi4_verify_draft", "qi4_last_error", "qi4_version",
 ]
 
 
@@ -137,34 +137,46 @@ def binding_path() -> Path:
 
 
 def build_torch_binding(force: bool = False) -> Path:
-    """Compile csrc/torch_binding.cpp (the C++ fast path of the Python
-    QuantLinear call) against this interpreter's torch and libqi4_b200.so,
-    in-tree next to the library. Rebuilt when the source, the C header or the
-    library is newer than the module."""
+    """Compile csrc/*.cpp (the C++ side of the Python calls: the QuantLinear
+    fast path and the paged-cache operators) against this interpreter's torch
+    and libqi4_b200.so, in-tree next to the library. A source is recompiled
+    when it or the C header is newer than its object."""
     import sysconfig
 
     import torch
 
-    src = CSRC / "torch_binding.cpp"
+    header = ROOT / "include" / "qi4_b200.h"
     out = binding_path()
-    deps = [src, ROOT / "include" / "qi4_b200.h", LIB]
-    if not force and out.exists() and out.stat().st_mtime >= max(d.stat().st_mtime for d in deps):
-        return out
+    BUILD.mkdir(exist_ok=True)
     torch_dir = Path(torch.__file__).resolve().parent
     cuda_home = Path(nvcc()).resolve().parent.parent
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_EXTENSION_NAME=_qi4_torch", "-DTORCH_API_INCLUDE_EXTENSION_H",
-           "-I", str(torch_dir / "include"), "-I", str(torch_dir / "include" / "torch" / "csrc" / "api" / "include"),
-           "-I", sysconfig.get_paths()["include"], "-I", str(cuda_home / "include"), "-I", str(ROOT / "include"),
-           str(src), "-o", str(out) + ".tmp",
-           "-L", str(torch_dir / "lib"), "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_cuda",
-           "-L", str(PKG), "-lqi4_b200", "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + str(torch_dir / "lib")]
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    (BUILD / "torch_binding.log").write_text(" ".join(cmd) + "\n" + proc.stdout + proc.stderr)
-    if proc.returncode != 0:
-        raise RuntimeError(f"torch binding build failed:\n{proc.stderr[-4000:]}")
-    os.replace(str(out) + ".tmp", out)
+    gxx = shutil.which("g++") or "g++"
+    flags = ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+             "-DTORCH_EXTENSION_NAME=_qi4_torch", "-DTORCH_API_INCLUDE_EXTENSION_H", "-I", str(torch_dir / "include"),
+             "-I", str(torch_dir / "include" / "torch" / "csrc" / "api" / "include"),
+             "-I", sysconfig.get_paths()["include"], "-I", str(cuda_home / "include"), "-I", str(ROOT / "include")]
+
+    def run(cmd: list[str], log: Path) -> None:
+        proc = subprocess.run(cmd, capture_output=True, text=True)
+        log.write_text(" ".join(cmd) + "\n" + proc.stdout + proc.stderr)
+        if proc.returncode != 0:
+            raise RuntimeError(f"torch binding build failed:\n{proc.stderr[-4000:]}")
+
+    jobs, objects = [], []
+    for src in sorted(CSRC.glob("*.cpp")):
+        obj = BUILD / (src.stem + ".cpp.o")
+        objects.append(obj)
+        if force or not obj.exists() or obj.stat().st_mtime < max(src.stat().st_mtime, header.stat().st_mtime):
+            jobs.append(([gxx, *flags, "-c", str(src), "-o", str(obj)], BUILD / (src.stem + ".log")))
+    if jobs:
+        with ThreadPoolExecutor(max_workers=len(jobs)) as pool:
+            list(pool.map(lambda j: run(*j), jobs))
+    if jobs or not out.exists() or out.stat().st_mtime < max(d.stat().st_mtime for d in [*objects, LIB]):
+        run([gxx, "-shared", *map(str, objects), "-o", str(out) + ".tmp", "-L", str(torch_dir / "lib"), "-ltorch",
+             "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_cuda", "-L", str(PKG), "-lqi4_b200",
+             "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + str(torch_dir / "lib")], BUILD / "torch_binding_link.log")
+        os.replace(str(out) + ".tmp", out)
     return out
 
 

@@ -15,12 +15,16 @@
 #include "gemm_tc.cuh"
 #include "gemv.cuh"
 #include "gemv_mma.cuh"
+#include "paged.cuh"
 #include "peer_exchange.cuh"
 #include "qi4_common.cuh"
 
 namespace qi4 {
 int read_chain_error(cudaStream_t stream);      // decode_chain.cu
 int read_attention_error(cudaStream_t stream);  // attention.cu
+int read_append_error(cudaStream_t stream);     // paged_append.cu
+int read_paged_error(cudaStream_t stream);      // paged_attention.cu
+int read_verify_error(cudaStream_t stream);     // verify_draft.cu
 }
 
 namespace qi4 {
@@ -74,6 +78,25 @@ int current_device(DeviceInfo& info) {
 }
 
 }  // namespace
+
+int require_device(int* sms) {
+  DeviceInfo info;
+  const int rc = current_device(info);
+  *sms = info.sms;
+  return rc;
+}
+
+int read_error_word(const void* symbol, cudaStream_t stream) {
+  int v = 0;
+  if (cudaMemcpyFromSymbolAsync(&v, symbol, sizeof(int), 0, cudaMemcpyDeviceToHost, stream) != cudaSuccess) return -1;
+  if (cudaStreamSynchronize(stream) != cudaSuccess) return -1;
+  if (v) {
+    const int zero = 0;
+    cudaMemcpyToSymbolAsync(symbol, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, stream);
+    cudaStreamSynchronize(stream);
+  }
+  return v;
+}
 
 // One pool per device, created on first use and kept for the life of the
 // process (the pool handle belongs to the device context current then: a
@@ -749,7 +772,12 @@ int qi4_device_status(void* stream) {
   const int v3 = read_chain_error(static_cast<cudaStream_t>(stream));
   const int v4 = read_attention_error(static_cast<cudaStream_t>(stream));
   const int v5 = read_peer_error(static_cast<cudaStream_t>(stream));
-  const int v = (v1 < 0 || v2 < 0 || v3 < 0 || v4 < 0 || v5 < 0) ? -1 : (v1 | v2 | v3 | v4 | v5);
+  const int v6 = read_append_error(static_cast<cudaStream_t>(stream));
+  const int v7 = read_paged_error(static_cast<cudaStream_t>(stream));
+  const int v8 = read_verify_error(static_cast<cudaStream_t>(stream));
+  const int v = (v1 < 0 || v2 < 0 || v3 < 0 || v4 < 0 || v5 < 0 || v6 < 0 || v7 < 0 || v8 < 0)
+                    ? -1
+                    : (v1 | v2 | v3 | v4 | v5 | v6 | v7 | v8);
   if (v < 0) {
     set_error("cannot read the device error flags: %s", cudaGetErrorString(cudaGetLastError()));
     return QI4_ERR_LAUNCH;

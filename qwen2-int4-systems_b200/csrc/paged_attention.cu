@@ -1,0 +1,638 @@
+// Attention of a ragged batch's new tokens over a paged KV cache (sm_100a):
+//   out[t, h] = sum_j w_j V[j] / sum_j w_j,   w_j = exp(scale q[t, h] . K[j])
+// over the keys j the token sees (causal: token i of n sees keys up to
+// length - n + i). Work split and merging: paged_attention.cuh.
+//
+// This kernel serves rows that are few per key (decode steps, drafts): it is
+// bound by the one pass over the keys and values. One CTA per SM; a producer
+// warp fetches units of 128 keys page by page (one TMA box per page and 64
+// dimensions, 128-byte swizzle) into a ring of 64 KB (D = 128) stages, three
+// of them: 192 KB in flight per SM, four times what the HBM latency asks for.
+// Eight warps take 16 keys each on mma.sync, keys as the 16 rows and the query
+// rows as columns of 8, so 6 query heads of a KV head waste 2 columns and not
+// 10. Scores S^T = K Q^T, a softmax with running max per warp on the score
+// registers, O^T += V^T P^T with P split into a 16-bit value and its 16-bit
+// remainder (the products keep 16 bits or more of each weight; the second
+// product is hidden behind the loads). The warps' sums meet in the stage of
+// the item's last unit, which is released afterwards.
+#include <algorithm>
+#include <atomic>
+#include <chrono>
+
+#include "paged_attention.cuh"
+
+namespace qi4 {
+
+__device__ int g_paged_error;
+
+namespace {
+
+constexpr int kWarps = 8;                        // consumer warps
+constexpr int kThreads = 32 * (kWarps + 1);      // and the producer
+constexpr int stages_of(int D) { return D == 128 ? 3 : 6; }
+constexpr int stage_bytes(int D) { return 2 * kBlockKeys * D * 2; }
+constexpr size_t smem_of(int D, int NT) {
+  return 1024 + (size_t)stages_of(D) * stage_bytes(D) + (size_t)8 * NT * (2 * D + 16) +
+         2 * 2 * kWarps * 8 * NT * sizeof(float) + 2 * stages_of(D) * sizeof(uint64_t) + 16;
+}
+
+template <bool F16>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (F16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
+  return d;
+}
+template <bool F16>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if constexpr (F16) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+// One box {64 dims, rows, one head, one page} of the pool into shared memory.
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int slot, int head, int page,
+                                         uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(slot), "r"(head), "r"(page), "r"(smem_addr(bar))
+      : "memory");
+}
+
+template <int D, int NT, bool F16>
+__global__ void __launch_bounds__(kThreads, 1)
+    paged_decode_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                        const PagedArgs a) {
+  constexpr int R = 8 * NT;
+  constexpr int kStages = stages_of(D), kStageBytes = stage_bytes(D), kHalfBytes = kBlockKeys * 128;
+  constexpr int kQRow = 2 * D + 16;  // bytes of a staged query row (padded: conflict-free)
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
+  uint8_t* q_s = smem + kStages * kStageBytes;
+  float* red_m = reinterpret_cast<float*>(q_s + R * kQRow);  // [2][kWarps][R]
+  float* red_l = red_m + 2 * kWarps * R;
+  uint64_t* full = reinterpret_cast<uint64_t*>(red_l + 2 * kWarps * R);
+  uint64_t* empty = full + kStages;
+  int* last_s = reinterpret_cast<int*>(empty + kStages);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], kWarps);
+    }
+    fence_barrier_init();
+    prefetch_tensor_map(&kmap);
+    prefetch_tensor_map(&vmap);
+  }
+  __syncthreads();
+  // The next launch may be scheduled once every CTA has passed its own wait:
+  // what it reads before its wait is then older than this launch.
+  pdl_wait();
+  pdl_launch_dependents();
+
+  Walk<R> w;
+  if (!w.begin(a, lane)) return;
+  int stage = 0;
+  uint32_t phase = 0;
+
+  if (warp == kWarps) {
+    // ---- producer: pages -> ring ----
+    const int box_rows = 1 << a.box_shift;
+    while (w.next(a)) {
+      const int vis = w.tile_visible(a);
+      const int nload = w.loaded(vis);
+      if (lane == 0 && a.fixed_len < 0 && __ldg(a.r.lengths + w.b) > a.cap) atomicOr(&g_paged_error, kErrCacheFull);
+      int win0 = -1, win = -1;  // table entries win0 .. win0 + 31, one per lane
+      for (int i = 0; i < nload; ++i) {
+        const int key0 = (w.blk + i) * kBlockKeys;
+        const int nb = (min(kBlockKeys, vis - key0) + box_rows - 1) >> a.box_shift;  // boxes per 64 dims
+        const int pj = key0 >> a.page_shift, slot = key0 & ((1 << a.page_shift) - 1);
+        if ((pj & ~31) != win0) {
+          win0 = pj & ~31;
+          const int j = win0 + lane;
+          win = j < a.table_width ? __ldg(a.table + w.b * a.table_stride + j) : -1;
+        }
+        mbar_wait(&empty[stage], phase ^ 1u, &g_paged_error);
+        const int boxes = 2 * (D / 64) * nb;
+        if (lane == 0) mbar_arrive_expect_tx(&full[stage], (uint32_t)(boxes * box_rows * 128));
+        __syncwarp();
+        const uint32_t base = smem_addr(smem + stage * kStageBytes);
+        for (int j0 = 0; j0 < boxes; j0 += 32) {
+          const int j = j0 + lane;
+          const int bx = j / (2 * (D / 64)), part = j - bx * (2 * (D / 64));  // part: K or V, 64-dim half
+          const int page = __shfl_sync(0xffffffffu, win, (pj + min(bx, nb - 1)) & 31);
+          if (j < boxes) {
+            // A page outside the pool reads as zeros (the copy's own bounds), and is reported.
+            if (part == 0 && (page < 0 || page >= a.pages)) atomicOr(&g_paged_error, kErrBadPage);
+            load_box(base + part * kHalfBytes + (bx << a.box_shift) * 128, part < D / 64 ? &kmap : &vmap,
+                     (part % (D / 64)) * 64, slot, w.kvh, page, &full[stage]);
+          }
+        }
+        if (++stage == kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+    return;
+  }
+
+  // ---- consumers ----
+  const int gq = lane >> 2, tq = lane & 3;
+  const int r0 = warp * 16;  // this warp's keys of every unit
+  const int lrow = r0 + (lane & 7) + (((lane >> 3) & 1) << 3), lchunk = lane >> 4, lx = lane & 7;
+  int par = 0;
+  while (w.next(a)) {
+    const int rows = w.rows(a), vis = w.tile_visible(a), nload = w.loaded(vis);
+    const int row0 = w.tile * R;
+    if (nload == 0 && !w.whole()) {
+      // A piece without visible keys still counts; its rows hold nothing.
+      float* slot = a.ws + (int64_t)w.slot(w.c) * (R * (D + 2));
+      for (int i = threadIdx.x; i < R * D / 4; i += 32 * kWarps)
+        reinterpret_cast<float4*>(slot)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int i = threadIdx.x; i < R; i += 32 * kWarps)
+        reinterpret_cast<float2*>(slot + R * D)[i] = make_float2(-INFINITY, 0.f);
+    } else if (nload == 0) {
+      for (int i = threadIdx.x; i < rows * (D / 4); i += 32 * kWarps) {
+        const int r = i / (D / 4), row = row0 + r;
+        finish_row<D, F16>(a, w.s.first + row / a.G, w.kvh * a.G + row % a.G, (i - r * (D / 4)) * 4,
+                           make_float4(0.f, 0.f, 0.f, 0.f), -INFINITY, 0.f);
+      }
+    }
+    if (nload > 0) {
+      // The tile's queries (rows past the last are zero).
+      for (int i = threadIdx.x; i < R * (D / 8); i += 32 * kWarps) {
+        const int r = i / (D / 8), ch = i - r * (D / 8), row = row0 + r;
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (r < rows)
+          v = *reinterpret_cast<const uint4*>(a.q + (int64_t)(w.s.first + row / a.G) * a.q_tok +
+                                              (int64_t)(w.kvh * a.G + row % a.G) * a.q_head + ch * 8);
+        sts128(smem_addr(q_s) + r * kQRow + ch * 16, v);
+      }
+      named_barrier(1, 32 * kWarps);
+      uint32_t qf[NT == 1 ? D / 16 : 1][2];
+      const uint32_t q_addr = smem_addr(q_s) + (lane & 7) * kQRow + (lane >> 3) * 16;
+      if constexpr (NT == 1) {
+#pragma unroll
+        for (int ks = 0; ks < D / 32; ++ks) {
+          ldsm4(q_addr + ks * 64, qf[2 * ks][0], qf[2 * ks][1], qf[2 * ks + 1][0], qf[2 * ks + 1][1]);
+        }
+      }
+      int lim[NT][2];  // keys that query row nt * 8 + 2 tq + e sees
+      int lim_min = vis;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = nt * 8 + 2 * tq + e;
+          lim[nt][e] = r < rows ? visible(a, w.s, row0 + r) : 0;
+          if (r < rows) lim_min = min(lim_min, lim[nt][e]);
+        }
+      lim_min = __reduce_min_sync(0xffffffffu, lim_min);
+      float m[NT][2], l[NT][2], o[D / 16][NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        m[nt][0] = m[nt][1] = -INFINITY;
+        l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+        for (int mt = 0; mt < D / 16; ++mt) o[mt][nt][0] = o[mt][nt][1] = o[mt][nt][2] = o[mt][nt][3] = 0.f;
+      }
+      int held = 0;
+      for (int i = 0; i < nload; ++i) {
+        const int key0 = (w.blk + i) * kBlockKeys + r0;
+        mbar_wait(&full[stage], phase, &g_paged_error);
+        const uint32_t kb = smem_addr(smem + stage * kStageBytes) + lrow * 128;
+        const uint32_t vb = kb + (D / 64) * kHalfBytes;
+        if (key0 < vis) {
+          if (key0 + 16 > vis) {
+            // Slots past the last key may hold anything: their values are
+            // zeroed, as a weight of zero times a NaN is not zero.
+            for (int j = lane; j < 16 * (D / 8); j += 32) {
+              const int r = j / (D / 8), ch = j - r * (D / 8);
+              if (key0 + r >= vis)
+                sts128(smem_addr(smem + stage * kStageBytes) + (D / 64 + (ch >> 3)) * kHalfBytes + (r0 + r) * 128 +
+                           ((ch & 7) << 4), make_uint4(0u, 0u, 0u, 0u));
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          float sc[NT][4];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+#pragma unroll
+          for (int k2 = 0; k2 < D / 32; ++k2) {
+            uint32_t ka[2][4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int ch = (2 * k2 + h) * 2 + lchunk;
+              ldsm4(kb + (ch >> 3) * kHalfBytes + (((ch & 7) ^ lx) << 4), ka[h][0], ka[h][1], ka[h][2], ka[h][3]);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              uint32_t q0, q1, q2, q3;
+              if constexpr (NT == 1) {
+                q0 = qf[2 * k2][0], q1 = qf[2 * k2][1], q2 = qf[2 * k2 + 1][0], q3 = qf[2 * k2 + 1][1];
+              } else {
+                ldsm4(q_addr + nt * 8 * kQRow + k2 * 64, q0, q1, q2, q3);
+              }
+              mma16816<F16>(sc[nt], ka[0], q0, q1);
+              mma16816<F16>(sc[nt], ka[1], q2, q3);
+            }
+          }
+          uint32_t ph[NT][2], pl[NT][2];
+          const bool masked = key0 + 16 > lim_min;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float alpha[2], p[4];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float x0 = sc[nt][e] * a.scale_log2, x1 = sc[nt][2 + e] * a.scale_log2;
+              if (masked || lim[nt][e] == 0) {
+                x0 = key0 + gq < lim[nt][e] ? x0 : -INFINITY;
+                x1 = key0 + gq + 8 < lim[nt][e] ? x1 : -INFINITY;
+              }
+              float t = fmaxf(x0, x1);
+              t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
+              t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
+              t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
+              const float mn = fmaxf(m[nt][e], t);
+              const float base = mn == -INFINITY ? 0.f : mn;
+              alpha[e] = exp2_approx(m[nt][e] - base);
+              m[nt][e] = mn;
+              p[e] = exp2_approx(x0 - base);
+              p[2 + e] = exp2_approx(x1 - base);
+              l[nt][e] = l[nt][e] * alpha[e] + (p[e] + p[2 + e]);  // this lane's keys; summed over gq at the end
+            }
+#pragma unroll
+            for (int mt = 0; mt < D / 16; ++mt) {
+              o[mt][nt][0] *= alpha[0];
+              o[mt][nt][1] *= alpha[1];
+              o[mt][nt][2] *= alpha[0];
+              o[mt][nt][3] *= alpha[1];
+            }
+            const uint32_t h0 = pack2<F16>(p[0], p[1]), h1 = pack2<F16>(p[2], p[3]);
+            const float2 f0 = unpack2<F16>(h0), f1 = unpack2<F16>(h1);
+            ph[nt][0] = transpose8x8(h0);
+            ph[nt][1] = transpose8x8(h1);
+            pl[nt][0] = transpose8x8(pack2<F16>(p[0] - f0.x, p[1] - f0.y));
+            pl[nt][1] = transpose8x8(pack2<F16>(p[2] - f1.x, p[3] - f1.y));
+          }
+#pragma unroll
+          for (int mt = 0; mt < D / 16; ++mt) {
+            uint32_t va[4];
+            const int ch = mt * 2 + lchunk;
+            ldsm4_t(vb + (ch >> 3) * kHalfBytes + (((ch & 7) ^ lx) << 4), va[0], va[2], va[1], va[3]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma16816<F16>(o[mt][nt], va, ph[nt][0], ph[nt][1]);
+              mma16816<F16>(o[mt][nt], va, pl[nt][0], pl[nt][1]);
+            }
+          }
+        }
+        if (i + 1 < nload) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&empty[stage]);
+        } else {
+          held = stage;  // the last unit's stage becomes the buffer of the reduction below
+        }
+        if (++stage == kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      // ---- the warps' sums ----
+      float* rm = red_m + par * kWarps * R;
+      float* rl = red_l + par * kWarps * R;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float t = l[nt][e];
+          t += __shfl_xor_sync(0xffffffffu, t, 4);
+          t += __shfl_xor_sync(0xffffffffu, t, 8);
+          t += __shfl_xor_sync(0xffffffffu, t, 16);
+          if (gq == 0) {
+            rm[warp * R + nt * 8 + 2 * tq + e] = m[nt][e];
+            rl[warp * R + nt * 8 + 2 * tq + e] = t;
+          }
+        }
+      named_barrier(1, 32 * kWarps);  // every warp is done with the held stage
+      // Four buffers [R][D], dims swizzled so that the fragments' stores spread over the banks.
+      float* buf = reinterpret_cast<float*>(smem + held * kStageBytes);
+      static_assert(4 * R * D * sizeof(float) <= (size_t)stage_bytes(D), "the sums must fit one stage");
+      float f[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int x = 0; x < kWarps; ++x) top = fmaxf(top, rm[x * R + nt * 8 + 2 * tq + e]);
+          f[nt][e] = m[nt][e] == -INFINITY ? 0.f : exp2_approx(m[nt][e] - top);
+        }
+      float* mine = buf + (warp & 3) * R * D;
+#pragma unroll
+      for (int round = 0; round < 2; ++round) {
+        if ((warp >= 4) == (round == 0)) {
+#pragma unroll
+          for (int mt = 0; mt < D / 16; ++mt)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const int r = nt * 8 + 2 * tq + (x & 1), d = mt * 16 + gq + (x >> 1) * 8;
+                float* at = mine + r * D + (d ^ (tq << 3));
+                const float v = o[mt][nt][x] * f[nt][x & 1];
+                *at = round == 0 ? v : *at + v;
+              }
+        }
+        named_barrier(1, 32 * kWarps);
+      }
+      constexpr int kLanes = D / 4;
+      const bool whole = w.whole();
+      float* slot = whole ? nullptr : a.ws + (int64_t)w.slot(w.c) * (R * (D + 2));
+      for (int i = threadIdx.x; i < rows * kLanes; i += 32 * kWarps) {
+        const int r = i / kLanes, d = (i - r * kLanes) * 4;
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int x = 0; x < kWarps; ++x) top = fmaxf(top, rm[x * R + r]);
+#pragma unroll
+        for (int x = 0; x < kWarps; ++x)
+          sum += rm[x * R + r] == -INFINITY ? 0.f : rl[x * R + r] * exp2_approx(rm[x * R + r] - top);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const float4 v = *reinterpret_cast<const float4*>(buf + (x * R + r) * D + (d ^ (((r >> 1) & 3) << 3)));
+          acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+        }
+        if (whole) {
+          const int row = row0 + r;
+          finish_row<D, F16>(a, w.s.first + row / a.G, w.kvh * a.G + row % a.G, d, acc, top, sum);
+        } else {
+          *reinterpret_cast<float4*>(slot + r * D + d) = acc;
+          if (d == 0) *reinterpret_cast<float2*>(slot + R * D + 2 * r) = make_float2(top, sum);
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[held]);
+      par ^= 1;
+    }
+    if (!w.whole()) {
+      __threadfence();
+      named_barrier(1, 32 * kWarps);
+      if (threadIdx.x == 0) *last_s = arrive_last(a.counters + w.first_cta(), a.call, w.pieces());
+      named_barrier(1, 32 * kWarps);
+      if (*last_s) {
+        __threadfence();
+        merge_pieces<D, R, F16>(a, w, warp, kWarps, lane);
+      }
+    }
+  }
+}
+
+}  // namespace
+
+int read_paged_error(cudaStream_t stream) { return read_error_word(&g_paged_error, stream); }
+
+namespace {
+
+template <int D, int NT, bool F16>
+cudaError_t launch_decode(const CUtensorMap& k, const CUtensorMap& v, const PagedArgs& a, int ctas, cudaStream_t s) {
+  auto kernel = paged_decode_kernel<D, NT, F16>;
+  static std::atomic<unsigned long long> configured{0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (!(configured.load(std::memory_order_relaxed) & bit)) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_of(D, NT));
+    if (e != cudaSuccess) return e;
+    configured.fetch_or(bit, std::memory_order_relaxed);
+  }
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas, 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = smem_of(D, NT);
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, k, v, a);
+}
+
+template <int D, bool F16>
+cudaError_t launch_rows(int nt, const CUtensorMap& k, const CUtensorMap& v, const PagedArgs& a, int ctas,
+                        cudaStream_t s) {
+  if (nt == 1) return launch_decode<D, 1, F16>(k, v, a, ctas, s);
+  if (nt == 2) return launch_decode<D, 2, F16>(k, v, a, ctas, s);
+  return launch_decode<D, 4, F16>(k, v, a, ctas, s);
+}
+
+cudaError_t launch_kernel(int D, bool f16, int nt, const CUtensorMap& k, const CUtensorMap& v, const PagedArgs& a,
+                          int ctas, cudaStream_t s) {
+  if (D == 128) return f16 ? launch_rows<128, true>(nt, k, v, a, ctas, s) : launch_rows<128, false>(nt, k, v, a, ctas, s);
+  return f16 ? launch_rows<64, true>(nt, k, v, a, ctas, s) : launch_rows<64, false>(nt, k, v, a, ctas, s);
+}
+
+constexpr int kMaxRows = 32;  // rows of a tile at most
+
+size_t pieces_bytes(int D, int ctas) { return (size_t)ctas * (2 * kMaxRows * (D + 2) * sizeof(float) + 8); }
+size_t state_bytes(int64_t T, int64_t Hq, int D) { return (size_t)(T * Hq) * (D + 2) * sizeof(float); }
+
+// A number no other call of this process bears, and hardly one of another
+// process: the counters' words start from the clock.
+unsigned long long next_call() {
+  static std::atomic<unsigned long long> n{
+      (unsigned long long)std::chrono::steady_clock::now().time_since_epoch().count()};
+  const unsigned long long v = n.fetch_add(1, std::memory_order_relaxed) & ((1ull << 48) - 1);
+  return v ? v : 1;
+}
+
+struct Call {
+  const qi4_paged_kv* kv;
+  const void* q;
+  int64_t q_tok, q_head;
+  void* out;
+  int64_t T, B, Hq;
+  const int32_t* cu;
+  const int32_t* lengths;
+  int64_t max_tokens;
+  float scale;
+  int causal;
+  const int32_t* prefix_table;
+  int64_t prefix_width, prefix_len;
+  void* ws;
+  size_t ws_bytes;
+  cudaStream_t stream;
+};
+
+int attend(const Call& c, const char* what) {
+  clear_error();
+  int rc = check_paged_kv(c.kv, what);
+  if (rc) return rc;
+  const qi4_paged_kv& kv = *c.kv;
+  if (c.T < 0 || c.B <= 0 || c.T > (1ll << 30) || c.B > (1ll << 30) || c.Hq <= 0 || c.Hq > 65535 || c.max_tokens < 0) {
+    set_error("%s: B and Hq must be positive, T and max_tokens not negative", what);
+    return QI4_ERR_ARGUMENT;
+  }
+  if (c.T == 0) return QI4_OK;
+  if (!c.q || !c.out || !c.lengths) {
+    set_error("%s: q, out and lengths must be non-null", what);
+    return QI4_ERR_ARGUMENT;
+  }
+  if (!c.cu && c.T % c.B) {
+    set_error("%s: without cu_tokens every sequence has T / B tokens (got T = %lld, B = %lld)", what, (long long)c.T,
+              (long long)c.B);
+    return QI4_ERR_SHAPE;
+  }
+  if ((kv.head_dim != 64 && kv.head_dim != 128) || c.Hq % kv.kv_heads) {
+    set_error("%s supports head_dim 64 and 128 and query heads that are a multiple of the KV heads (got %d, %lld/%d)",
+              what, kv.head_dim, (long long)c.Hq, kv.kv_heads);
+    return QI4_ERR_SHAPE;
+  }
+  if (c.T * c.Hq >= (1ll << 31)) {
+    set_error("%s: at most 2^31 rows (tokens x query heads)", what);
+    return QI4_ERR_SHAPE;
+  }
+  auto al = [](const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
+  if (!al(c.q, 16) || !al(c.out, 16) || c.q_tok % 8 || c.q_head % 8 || c.q_tok < 0 || c.q_head < 0) {
+    set_error("%s: q and out must be 16-byte aligned, q with strides that are multiples of 8 elements", what);
+    return QI4_ERR_ALIGNMENT;
+  }
+  const bool prefix = c.prefix_len > 0;
+  if (c.prefix_len < 0 || (prefix && (!c.prefix_table || c.prefix_width <= 0))) {
+    set_error("%s: a prefix needs its page table and a length that is not negative", what);
+    return QI4_ERR_ARGUMENT;
+  }
+  if (prefix && c.prefix_len > c.prefix_width * kv.page_size) {
+    set_error("%s: the prefix is longer (%lld) than its page table covers", what, (long long)c.prefix_len);
+    return QI4_ERR_SHAPE;
+  }
+  int sms = 0;
+  rc = require_device(&sms);
+  if (rc) return rc;
+  const int D = kv.head_dim;
+  const size_t pieces = (pieces_bytes(D, sms) + 255) / 256 * 256;
+  const size_t need = (prefix ? 2 : 1) * pieces + (prefix ? state_bytes(c.T, c.Hq, D) : 0);
+  char* ws = static_cast<char*>(c.ws);
+  if (ws && (c.ws_bytes < need || !al(ws, 16))) {
+    set_error("%s: the workspace needs %zu bytes, 16-byte aligned (got %zu)", what, need, c.ws_bytes);
+    return QI4_ERR_ARGUMENT;
+  }
+  CUtensorMap kmap, vmap;
+  const uint32_t box_rows = (uint32_t)std::min(kv.page_size, kBlockKeys);
+  if (!tensor_map_pages(&kmap, kv.k, kv, box_rows) || !tensor_map_pages(&vmap, kv.v, kv, box_rows)) return QI4_ERR_LAUNCH;
+  void* own = nullptr;
+  if (!ws) {
+    if (scratch_alloc(&own, need, c.stream) != cudaSuccess) {
+      cudaGetLastError();
+      set_error("%s: cannot allocate %zu bytes of scratch", what, need);
+      return QI4_ERR_LAUNCH;
+    }
+    ws = static_cast<char*>(own);
+  }
+  PagedArgs a = {};
+  a.q = static_cast<const uint16_t*>(c.q);
+  a.q_tok = c.q_tok, a.q_head = c.q_head;
+  a.out = static_cast<uint16_t*>(c.out);
+  a.page_shift = __builtin_ctz((unsigned)kv.page_size), a.box_shift = __builtin_ctz(box_rows);
+  a.pages = kv.pages;
+  a.Hkv = kv.kv_heads, a.G = (int)(c.Hq / kv.kv_heads);
+  a.scale_log2 = c.scale * 1.4426950408889634f;
+  const bool f16 = kv.dtype == QI4_DTYPE_F16;
+  cudaError_t e = cudaSuccess;
+  auto pieces_at = [&](PagedArgs& x, char* p) {
+    x.ws = reinterpret_cast<float*>(p);
+    x.counters = reinterpret_cast<unsigned long long*>(p + (size_t)sms * 2 * kMaxRows * (D + 2) * sizeof(float));
+    x.call = next_call();
+  };
+  // Rows per tile: the smallest of 8, 16 and 32 that holds a sequence's rows.
+  auto tiles = [](int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; };
+  float* state = nullptr;
+  if (prefix) {
+    // All tokens as one sequence over the prefix, each row seeing all of it.
+    state = reinterpret_cast<float*>(ws + 2 * pieces);
+    PagedArgs p = a;
+    pieces_at(p, ws + pieces);
+    p.table = c.prefix_table, p.table_stride = 0, p.table_width = (int)c.prefix_width;
+    p.r = {nullptr, nullptr, 1, (int)c.T, (int)c.T};
+    p.fixed_len = (int)c.prefix_len, p.cap = (int)c.prefix_len, p.causal = 0;
+    p.state_acc = state, p.state_ml = state + c.T * c.Hq * D;
+    e = launch_kernel(D, f16, tiles(c.T * a.G), kmap, vmap, p, sms, c.stream);
+  }
+  if (e == cudaSuccess) {
+    pieces_at(a, ws);
+    a.table = kv.block_table, a.table_stride = kv.table_stride, a.table_width = kv.table_width;
+    a.r = {c.cu, c.lengths, (int)c.B, (int)c.T, (int)(c.T / c.B)};
+    a.fixed_len = -1, a.cap = kv.table_width * kv.page_size, a.causal = c.causal;
+    if (prefix) a.prior_acc = state, a.prior_ml = state + c.T * c.Hq * D;
+    const int64_t most = c.cu ? (c.max_tokens ? std::min(c.max_tokens, c.T) : c.T) : c.T / c.B;
+    e = launch_kernel(D, f16, tiles(most * a.G), kmap, vmap, a, sms, c.stream);
+  }
+  if (own) scratch_free(own, c.stream);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    set_error("%s launch failed: %s", what, cudaGetErrorString(e));
+    return QI4_ERR_LAUNCH;
+  }
+  return QI4_OK;
+}
+
+}  // namespace
+}  // namespace qi4
+
+extern "C" QI4_API int qi4_paged_attention(const qi4_paged_kv* kv, const void* q, int64_t q_token_stride,
+                                           int64_t q_head_stride, void* out, int64_t T, int64_t B, int64_t Hq,
+                                           const int32_t* cu_tokens, const int32_t* lengths, int64_t max_tokens,
+                                           float scale, int causal, void* workspace, size_t workspace_bytes,
+                                           void* stream) {
+  return qi4::attend({kv, q, q_token_stride, q_head_stride, out, T, B, Hq, cu_tokens, lengths, max_tokens, scale,
+                      causal ? 1 : 0, nullptr, 0, 0, workspace, workspace_bytes, static_cast<cudaStream_t>(stream)},
+                     "paged attention");
+}
+
+extern "C" QI4_API int qi4_shared_prefix_attention(const qi4_paged_kv* kv, const void* q, int64_t q_token_stride,
+                                                   int64_t q_head_stride, void* out, int64_t T, int64_t B, int64_t Hq,
+                                                   const int32_t* prefix_table, int64_t prefix_pages,
+                                                   int64_t prefix_length, const int32_t* cu_tokens,
+                                                   const int32_t* lengths, int64_t max_tokens, float scale,
+                                                   void* workspace, size_t workspace_bytes, void* stream) {
+  return qi4::attend({kv, q, q_token_stride, q_head_stride, out, T, B, Hq, cu_tokens, lengths, max_tokens, scale, 1,
+                      prefix_table, prefix_pages, prefix_length, workspace, workspace_bytes,
+                      static_cast<cudaStream_t>(stream)},
+                     "shared-prefix attention");
+}
+
+extern "C" QI4_API size_t qi4_paged_attention_workspace(int64_t T, int64_t Hq, int head_dim, int prefix) {
+  if (T < 0 || Hq <= 0 || head_dim <= 0) return 0;
+  int sms = 0;
+  if (qi4::require_device(&sms)) return 0;
+  const size_t pieces = (qi4::pieces_bytes(head_dim, sms) + 255) / 256 * 256;
+  return (prefix ? 2 : 1) * pieces + (prefix ? qi4::state_bytes(T, Hq, head_dim) : 0);
+}

@@ -135,4 +135,32 @@ bool tensor_map_row_boxes(CUtensorMap* out, const void* base, uint64_t row_bytes
                        CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+bool tensor_map_pages(CUtensorMap* out, const void* base, const qi4_paged_kv& kv, uint32_t box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) {
+    set_error("cuTensorMapEncodeTiled is not available from the driver");
+    return false;
+  }
+  // (The stride of a dimension of size 1 is never used, but must be a valid one.)
+  auto stride = [](int64_t elements, int64_t count) { return (cuuint64_t)(count > 1 ? elements * 2 : 16); };
+  const cuuint64_t dims[4] = {(cuuint64_t)kv.head_dim, (cuuint64_t)kv.page_size, (cuuint64_t)kv.kv_heads,
+                              (cuuint64_t)kv.pages};
+  const cuuint64_t strides[3] = {stride(kv.slot_stride, kv.page_size), stride(kv.head_stride, kv.kv_heads),
+                                 stride(kv.page_stride, kv.pages)};
+  const cuuint32_t box[4] = {64, box_rows, 1, 1}, estr[4] = {1, 1, 1, 1};
+  alignas(64) CUtensorMap map;
+  const CUresult r = fn(&map, kv.dtype == QI4_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                        : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                        4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed (%d) for %d pages of %d x %d x %d", (int)r, kv.pages, kv.kv_heads,
+              kv.page_size, kv.head_dim);
+    return false;
+  }
+  *out = map;
+  return true;
+}
+
 }  // namespace qi4

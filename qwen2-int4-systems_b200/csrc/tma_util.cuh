@@ -13,6 +13,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "../../include/qi4_b200.h"
+
 namespace qi4 {
 
 // ---------------------------------------------------------------------------
@@ -31,6 +33,11 @@ bool tensor_map_2d(CUtensorMap* out, const void* base, CUtensorMapDataType dtype
 // [box_rows x 128 B] copies, in one request.
 bool tensor_map_row_boxes(CUtensorMap* out, const void* base, uint64_t row_bytes, uint64_t rows, uint32_t box_rows,
                           uint32_t boxes_per_copy);
+
+// The pages of a paged cache (16-bit elements) as a 4-D map (dims, slots of a
+// page, KV heads, pages) at the descriptor's strides, with a box of 64 dims x
+// box_rows slots and 128-byte swizzle. Encoded anew for every call.
+bool tensor_map_pages(CUtensorMap* out, const void* base, const qi4_paged_kv& kv, uint32_t box_rows);
 
 // Device-side error flags (one per translation unit), read and cleared on host.
 constexpr int kErrWaitTimeout = 1;

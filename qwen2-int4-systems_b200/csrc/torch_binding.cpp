@@ -134,9 +134,12 @@ at::Tensor linear(const at::Tensor& x, const at::Tensor& qweight, const at::Tens
 
 }  // namespace
 
+void bind_paged(py::module_& m);  // paged_binding.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
-  m.doc() = "C++ fast path of b200_w4g64_linear (checks + launch through the qi4 C ABI)";
+  m.doc() = "C++ entry points over the qi4 C ABI: b200_w4g64_linear and the paged-cache operators";
   m.def("linear", &linear, "Canonical W4G64 linear on the B200 kernels (same contract as b200_w4g64_linear)",
         py::arg("x"), py::arg("qweight"), py::arg("scales"), py::arg("zeros"), py::arg("bias"),
         py::arg("out_features"), py::arg("in_features"));
+  bind_paged(m);
 }
