@@ -472,8 +472,10 @@ QI4_API int qi4_shared_prefix_attention(const qi4_paged_kv* kv, const void* q, i
                                         const int32_t* cu_tokens, const int32_t* lengths, int64_t max_tokens,
                                         float scale, void* workspace, size_t workspace_bytes, void* stream);
 
-/* Workspace bytes of the two calls above on the current device (0 without one). */
-QI4_API size_t qi4_paged_attention_workspace(int64_t T, int64_t Hq, int head_dim, int prefix);
+/* Workspace bytes of the two calls above on the current device (0 without
+ * one). max_tokens as given to the call; without cu_tokens T / B. */
+QI4_API size_t qi4_paged_attention_workspace(int64_t T, int64_t Hq, int64_t kv_heads, int head_dim,
+                                             int64_t max_tokens, int prefix);
 
 /*
  * Verification of drafted tokens (speculative decoding) from given uniform

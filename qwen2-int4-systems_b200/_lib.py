@@ -61,7 +61,7 @@ SIGNATURES = {
     "qi4_paged_attention": [_p, _p, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _i64, ctypes.c_float, _i, _p, _sz, _p],
     "qi4_shared_prefix_attention": [_p, _p, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _i64,
                                     ctypes.c_float, _p, _sz, _p],
-    "qi4_paged_attention_workspace": [_i64, _i64, _i, _i],
+    "qi4_paged_attention_workspace": [_i64, _i64, _i64, _i, _i64, _i],
     "qi4_verify_draft": [_p, _p, _i64, _i64, _p, _i64, _i64, _i, _p, _p, _i64, _i64, _i64, _p, _p, _p],
     "qi4_last_error": [ctypes.c_char_p, _sz],
     "qi4_version": [],

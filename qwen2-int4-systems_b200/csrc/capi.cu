@@ -24,6 +24,7 @@ int read_chain_error(cudaStream_t stream);      // decode_chain.cu
 int read_attention_error(cudaStream_t stream);  // attention.cu
 int read_append_error(cudaStream_t stream);     // paged_append.cu
 int read_paged_error(cudaStream_t stream);      // paged_attention.cu
+int read_paged_tc_error(cudaStream_t stream);   // paged_prefill.cu
 int read_verify_error(cudaStream_t stream);     // verify_draft.cu
 }
 
@@ -775,9 +776,10 @@ int qi4_device_status(void* stream) {
   const int v6 = read_append_error(static_cast<cudaStream_t>(stream));
   const int v7 = read_paged_error(static_cast<cudaStream_t>(stream));
   const int v8 = read_verify_error(static_cast<cudaStream_t>(stream));
-  const int v = (v1 < 0 || v2 < 0 || v3 < 0 || v4 < 0 || v5 < 0 || v6 < 0 || v7 < 0 || v8 < 0)
+  const int v9 = read_paged_tc_error(static_cast<cudaStream_t>(stream));
+  const int v = (v1 < 0 || v2 < 0 || v3 < 0 || v4 < 0 || v5 < 0 || v6 < 0 || v7 < 0 || v8 < 0 || v9 < 0)
                     ? -1
-                    : (v1 | v2 | v3 | v4 | v5 | v6 | v7 | v8);
+                    : (v1 | v2 | v3 | v4 | v5 | v6 | v7 | v8 | v9);
   if (v < 0) {
     set_error("cannot read the device error flags: %s", cudaGetErrorString(cudaGetLastError()));
     return QI4_ERR_LAUNCH;

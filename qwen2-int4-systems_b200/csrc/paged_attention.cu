@@ -3,7 +3,8 @@
 // over the keys j the token sees (causal: token i of n sees keys up to
 // length - n + i). Work split and merging: paged_attention.cuh.
 //
-// This kernel serves rows that are few per key (decode steps, drafts): it is
+// This kernel serves rows that are few per key (decode steps, drafts; larger
+// counts go to paged_prefill.cu): it is
 // bound by the one pass over the keys and values. One CTA per SM; a producer
 // warp fetches units of 128 keys page by page (one TMA box per page and 64
 // dimensions, 128-byte swizzle) into a ring of 64 KB (D = 128) stages, three
@@ -71,16 +72,6 @@ __device__ __forceinline__ float2 unpack2(uint32_t w) {
   if constexpr (F16) return __half22float2(*reinterpret_cast<const __half2*>(&w));
   return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
 }
-// One box {64 dims, rows, one head, one page} of the pool into shared memory.
-__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int slot, int head, int page,
-                                         uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
-      "[%6];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(slot), "r"(head), "r"(page), "r"(smem_addr(bar))
-      : "memory");
-}
-
 template <int D, int NT, bool F16>
 __global__ void __launch_bounds__(kThreads, 1)
     paged_decode_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
@@ -177,19 +168,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         reinterpret_cast<float2*>(slot + R * D)[i] = make_float2(-INFINITY, 0.f);
     } else if (nload == 0) {
       for (int i = threadIdx.x; i < rows * (D / 4); i += 32 * kWarps) {
-        const int r = i / (D / 4), row = row0 + r;
-        finish_row<D, F16>(a, w.s.first + row / a.G, w.kvh * a.G + row % a.G, (i - r * (D / 4)) * 4,
-                           make_float4(0.f, 0.f, 0.f, 0.f), -INFINITY, 0.f);
+        const int r = i / (D / 4);
+        float none[4] = {0.f, 0.f, 0.f, 0.f};
+        finish_row<D, F16, 4>(a, w.token(a, r), w.head(a, r), (i - r * (D / 4)) * 4, none, -INFINITY, 0.f);
       }
     }
     if (nload > 0) {
       // The tile's queries (rows past the last are zero).
       for (int i = threadIdx.x; i < R * (D / 8); i += 32 * kWarps) {
-        const int r = i / (D / 8), ch = i - r * (D / 8), row = row0 + r;
+        const int r = i / (D / 8), ch = i - r * (D / 8);
         uint4 v = make_uint4(0u, 0u, 0u, 0u);
         if (r < rows)
-          v = *reinterpret_cast<const uint4*>(a.q + (int64_t)(w.s.first + row / a.G) * a.q_tok +
-                                              (int64_t)(w.kvh * a.G + row % a.G) * a.q_head + ch * 8);
+          v = *reinterpret_cast<const uint4*>(a.q + w.token(a, r) * a.q_tok + w.head(a, r) * a.q_head + ch * 8);
         sts128(smem_addr(q_s) + r * kQRow + ch * 16, v);
       }
       named_barrier(1, 32 * kWarps);
@@ -382,17 +372,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int x = 0; x < kWarps; ++x)
           sum += rm[x * R + r] == -INFINITY ? 0.f : rl[x * R + r] * exp2_approx(rm[x * R + r] - top);
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const float4 v = *reinterpret_cast<const float4*>(buf + (x * R + r) * D + (d ^ (((r >> 1) & 3) << 3)));
-          acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+          acc[0] += v.x, acc[1] += v.y, acc[2] += v.z, acc[3] += v.w;
         }
         if (whole) {
-          const int row = row0 + r;
-          finish_row<D, F16>(a, w.s.first + row / a.G, w.kvh * a.G + row % a.G, d, acc, top, sum);
+          finish_row<D, F16, 4>(a, w.token(a, r), w.head(a, r), d, acc, top, sum);
         } else {
-          *reinterpret_cast<float4*>(slot + r * D + d) = acc;
+          *reinterpret_cast<float4*>(slot + r * D + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
           if (d == 0) *reinterpret_cast<float2*>(slot + R * D + 2 * r) = make_float2(top, sum);
         }
       }
@@ -460,10 +449,21 @@ cudaError_t launch_kernel(int D, bool f16, int nt, const CUtensorMap& k, const C
   return f16 ? launch_rows<64, true>(nt, k, v, a, ctas, s) : launch_rows<64, false>(nt, k, v, a, ctas, s);
 }
 
-constexpr int kMaxRows = 32;  // rows of a tile at most
+// Rows of one sequence and KV head from which the tcgen05 kernel takes a batch.
+constexpr int64_t kTcFrom = 65;
+bool takes_tc(int64_t tokens, int64_t G) { return tokens * G >= kTcFrom && G <= 128; }
 
-size_t pieces_bytes(int D, int ctas) { return (size_t)ctas * (2 * kMaxRows * (D + 2) * sizeof(float) + 8); }
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+// Room for the pieces of a launch over `tokens` per sequence (and the counters).
+size_t pieces_bytes(int64_t tokens, int64_t G, int D, int ctas) {
+  const size_t rows = takes_tc(tokens, G) ? kTcRows : 32;
+  return round256((size_t)ctas * (2 * rows * (D + 2) * sizeof(float) + 8));
+}
 size_t state_bytes(int64_t T, int64_t Hq, int D) { return (size_t)(T * Hq) * (D + 2) * sizeof(float); }
+size_t workspace_bytes_for(int64_t T, int64_t Hq, int64_t Hkv, int D, int64_t most, bool prefix, int ctas) {
+  return pieces_bytes(most, Hq / Hkv, D, ctas) +
+         (prefix ? pieces_bytes(T, Hq / Hkv, D, ctas) + state_bytes(T, Hq, D) : 0);
+}
 
 // A number no other call of this process bears, and hardly one of another
 // process: the counters' words start from the clock.
@@ -538,8 +538,10 @@ int attend(const Call& c, const char* what) {
   rc = require_device(&sms);
   if (rc) return rc;
   const int D = kv.head_dim;
-  const size_t pieces = (pieces_bytes(D, sms) + 255) / 256 * 256;
-  const size_t need = (prefix ? 2 : 1) * pieces + (prefix ? state_bytes(c.T, c.Hq, D) : 0);
+  const int64_t G = c.Hq / kv.kv_heads;
+  // Tokens of a sequence at most, as far as the host knows.
+  const int64_t most = c.cu ? (c.max_tokens ? std::min(c.max_tokens, c.T) : c.T) : c.T / c.B;
+  const size_t need = workspace_bytes_for(c.T, c.Hq, kv.kv_heads, D, most, prefix, sms);
   char* ws = static_cast<char*>(c.ws);
   if (ws && (c.ws_bytes < need || !al(ws, 16))) {
     set_error("%s: the workspace needs %zu bytes, 16-byte aligned (got %zu)", what, need, c.ws_bytes);
@@ -567,33 +569,35 @@ int attend(const Call& c, const char* what) {
   a.scale_log2 = c.scale * 1.4426950408889634f;
   const bool f16 = kv.dtype == QI4_DTYPE_F16;
   cudaError_t e = cudaSuccess;
-  auto pieces_at = [&](PagedArgs& x, char* p) {
-    x.ws = reinterpret_cast<float*>(p);
-    x.counters = reinterpret_cast<unsigned long long*>(p + (size_t)sms * 2 * kMaxRows * (D + 2) * sizeof(float));
+  // One launch: pieces at `at`, the kernel for `tokens` per sequence. The
+  // mma.sync tile is the smallest of 8, 16 and 32 rows that holds them.
+  auto launch = [&](PagedArgs& x, char* at, int64_t tokens) {
+    const bool tc = takes_tc(tokens, G);
+    const size_t rows = tc ? kTcRows : 32;
+    x.ws = reinterpret_cast<float*>(at);
+    x.counters = reinterpret_cast<unsigned long long*>(at + (size_t)sms * 2 * rows * (D + 2) * sizeof(float));
     x.call = next_call();
+    if (tc) return launch_paged_tc(D, f16, kmap, vmap, x, sms, c.stream);
+    return launch_kernel(D, f16, tokens * G <= 8 ? 1 : tokens * G <= 16 ? 2 : 4, kmap, vmap, x, sms, c.stream);
   };
-  // Rows per tile: the smallest of 8, 16 and 32 that holds a sequence's rows.
-  auto tiles = [](int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; };
   float* state = nullptr;
   if (prefix) {
     // All tokens as one sequence over the prefix, each row seeing all of it.
-    state = reinterpret_cast<float*>(ws + 2 * pieces);
+    char* at = ws + pieces_bytes(most, G, D, sms);
+    state = reinterpret_cast<float*>(at + pieces_bytes(c.T, G, D, sms));
     PagedArgs p = a;
-    pieces_at(p, ws + pieces);
     p.table = c.prefix_table, p.table_stride = 0, p.table_width = (int)c.prefix_width;
     p.r = {nullptr, nullptr, 1, (int)c.T, (int)c.T};
     p.fixed_len = (int)c.prefix_len, p.cap = (int)c.prefix_len, p.causal = 0;
     p.state_acc = state, p.state_ml = state + c.T * c.Hq * D;
-    e = launch_kernel(D, f16, tiles(c.T * a.G), kmap, vmap, p, sms, c.stream);
+    e = launch(p, at, c.T);
   }
   if (e == cudaSuccess) {
-    pieces_at(a, ws);
     a.table = kv.block_table, a.table_stride = kv.table_stride, a.table_width = kv.table_width;
     a.r = {c.cu, c.lengths, (int)c.B, (int)c.T, (int)(c.T / c.B)};
     a.fixed_len = -1, a.cap = kv.table_width * kv.page_size, a.causal = c.causal;
     if (prefix) a.prior_acc = state, a.prior_ml = state + c.T * c.Hq * D;
-    const int64_t most = c.cu ? (c.max_tokens ? std::min(c.max_tokens, c.T) : c.T) : c.T / c.B;
-    e = launch_kernel(D, f16, tiles(most * a.G), kmap, vmap, a, sms, c.stream);
+    e = launch(a, ws, most);
   }
   if (own) scratch_free(own, c.stream);
   if (e != cudaSuccess) {
@@ -629,10 +633,10 @@ extern "C" QI4_API int qi4_shared_prefix_attention(const qi4_paged_kv* kv, const
                      "shared-prefix attention");
 }
 
-extern "C" QI4_API size_t qi4_paged_attention_workspace(int64_t T, int64_t Hq, int head_dim, int prefix) {
-  if (T < 0 || Hq <= 0 || head_dim <= 0) return 0;
+extern "C" QI4_API size_t qi4_paged_attention_workspace(int64_t T, int64_t Hq, int64_t kv_heads, int head_dim,
+                                                        int64_t max_tokens, int prefix) {
+  if (T < 0 || Hq <= 0 || kv_heads <= 0 || Hq % kv_heads || head_dim <= 0 || max_tokens < 0) return 0;
   int sms = 0;
   if (qi4::require_device(&sms)) return 0;
-  const size_t pieces = (qi4::pieces_bytes(head_dim, sms) + 255) / 256 * 256;
-  return (prefix ? 2 : 1) * pieces + (prefix ? qi4::state_bytes(T, Hq, head_dim) : 0);
+  return qi4::workspace_bytes_for(T, Hq, kv_heads, head_dim, max_tokens ? std::min(max_tokens, T) : T, prefix != 0, sms);
 }

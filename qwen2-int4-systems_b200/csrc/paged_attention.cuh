@@ -35,7 +35,7 @@ struct PagedArgs {
   int Hkv, G, cap;
   int causal;
   float scale_log2;  // scale * log2(e)
-  float* ws;         // pieces: kSlots per CTA, each R x D sums then R x (max, sum)
+  float* ws;         // pieces: two slots per CTA, each R x D sums then R x (max, sum)
   unsigned long long* counters;  // one per CTA
   unsigned long long call;       // number of this call, 1 .. 2^48 - 1
   // Keys that every row has seen already (a shared prefix): per row t * Hq + h
@@ -170,6 +170,8 @@ struct Walk {
   }
   __device__ __forceinline__ bool whole() const { return blk == 0 && nblk == s.blocks; }
   __device__ __forceinline__ int rows(const PagedArgs& a) const { return min(R, s.n * a.G - tile * R); }
+  __device__ __forceinline__ int64_t token(const PagedArgs& a, int r) const { return s.first + (tile * R + r) / a.G; }
+  __device__ __forceinline__ int head(const PagedArgs& a, int r) const { return kvh * a.G + (tile * R + r) % a.G; }
   // Keys the tile's last row sees: none beyond is loaded.
   __device__ __forceinline__ int tile_visible(const PagedArgs& a) const {
     return visible(a, s, tile * R + rows(a) - 1);
@@ -213,76 +215,100 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return d;
 }
 
-// Four dims (at d) of a finished row: weighted sums, max and sum of weights
-// over its own keys. Joins the prior state, and writes the output or the state.
-// A row that saw no key is zero.
-template <int D, bool F16>
-__device__ __forceinline__ void finish_row(const PagedArgs& a, int64_t token, int head, int d, float4 acc, float m,
+// N dims (at d) of a finished row: weighted sums, max and sum of weights over
+// its own keys. Joins the prior state, and writes the output or the state. A
+// row that saw no key is zero.
+template <int D, bool F16, int N>
+__device__ __forceinline__ void finish_row(const PagedArgs& a, int64_t token, int head, int d, float (&acc)[N], float m,
                                            float l) {
   const int64_t row = token * (a.Hkv * a.G) + head;
   if (a.state_acc) {
-    *reinterpret_cast<float4*>(a.state_acc + row * D + d) = acc;
+#pragma unroll
+    for (int i = 0; i < N; i += 4)
+      *reinterpret_cast<float4*>(a.state_acc + row * D + d + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
     if (d == 0) *reinterpret_cast<float2*>(a.state_ml + 2 * row) = make_float2(m, l);
     return;
   }
   if (a.prior_acc) {
-    const float4 pa = *reinterpret_cast<const float4*>(a.prior_acc + row * D + d);
     const float2 pm = *reinterpret_cast<const float2*>(a.prior_ml + 2 * row);
     const float top = fmaxf(m, pm.x);
     const float f = m == -INFINITY ? 0.f : exp2_approx(m - top), g = pm.x == -INFINITY ? 0.f : exp2_approx(pm.x - top);
-    acc = make_float4(acc.x * f + pa.x * g, acc.y * f + pa.y * g, acc.z * f + pa.z * g, acc.w * f + pa.w * g);
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const float4 p = *reinterpret_cast<const float4*>(a.prior_acc + row * D + d + i);
+      acc[i] = acc[i] * f + p.x * g;
+      acc[i + 1] = acc[i + 1] * f + p.y * g;
+      acc[i + 2] = acc[i + 2] * f + p.z * g;
+      acc[i + 3] = acc[i + 3] * f + p.w * g;
+    }
     l = l * f + pm.y * g;
   }
   const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
-  uint2 w;
-  w.x = pack2<F16>(acc.x * inv, acc.y * inv);
-  w.y = pack2<F16>(acc.z * inv, acc.w * inv);
-  *reinterpret_cast<uint2*>(a.out + row * D + d) = w;
+  uint32_t w[N / 2];
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) w[i] = pack2<F16>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+  if constexpr (N == 8)
+    *reinterpret_cast<uint4*>(a.out + row * D + d) = make_uint4(w[0], w[1], w[2], w[3]);
+  else
+    *reinterpret_cast<uint2*>(a.out + row * D + d) = make_uint2(w[0], w[1]);
 }
 
 // Merges the pieces of the walk's current item and finishes its rows: a group
-// of D / 4 lanes per row, `nwarps` warps. Pieces in the order of their CTAs.
-template <int D, int R, bool F16>
-__device__ __forceinline__ void merge_pieces(const PagedArgs& a, const Walk<R>& w, int warp, int nwarps, int lane) {
+// of D / 4 lanes per row, warp `warp` of `nwarps`. Pieces in the order of
+// their CTAs: the first CTA's, then the first slot of each later one.
+template <int D, int R, bool F16, class W>
+__device__ __forceinline__ void merge_pieces(const PagedArgs& a, const W& w, int warp, int nwarps, int lane) {
   constexpr int kLanes = D / 4, kPerWarp = 32 / kLanes;
   constexpr int64_t kSlot = (int64_t)R * (D + 2);
   const int np = w.pieces(), p0 = w.first_cta(), rows = w.rows(a);
+  const float* first = a.ws + w.slot(p0) * kSlot;
+  const float* later = a.ws + 2 * (int64_t)p0 * kSlot;  // piece p > 0 at later + 2 p kSlot
   const int d = (lane % kLanes) * 4;
   for (int r0 = warp * kPerWarp; r0 < rows; r0 += nwarps * kPerWarp) {
     const int r = min(r0 + lane / kLanes, rows - 1);
-    // Slots: the first CTA's own, then the first slot of each later one.
+    const int64_t at_ml = (int64_t)R * D + 2 * r, at_acc = (int64_t)r * D + d;
     float top = -INFINITY;
-    for (int p = lane % kLanes; p < np; p += kLanes)
-      top = fmaxf(top, __ldcg(a.ws + (p ? 2 * (int64_t)(p0 + p) : w.slot(p0)) * kSlot + (int64_t)R * D + 2 * r));
+    for (int p = lane % kLanes; p < np; p += kLanes) top = fmaxf(top, __ldcg((p ? later + 2 * p * kSlot : first) + at_ml));
 #pragma unroll
     for (int o = kLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
     float l = 0.f;
     for (int q0 = 0; q0 < np; q0 += kLanes) {
       const int p = q0 + lane % kLanes;
       float2 ml = make_float2(-INFINITY, 0.f);
-      if (p < np)
-        ml = __ldcg(reinterpret_cast<const float2*>(a.ws + (p ? 2 * (int64_t)(p0 + p) : w.slot(p0)) * kSlot +
-                                                    (int64_t)R * D + 2 * r));
+      if (p < np) ml = __ldcg(reinterpret_cast<const float2*>((p ? later + 2 * p * kSlot : first) + at_ml));
       const float fp = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - top);
       const float lp = ml.y * fp;
       const int cnt = min(kLanes, np - q0);
-#pragma unroll 8
+      const float* src = later + 2 * q0 * kSlot + at_acc;
+#pragma unroll 16
       for (int j = 0; j < cnt; ++j) {
         const float f = __shfl_sync(0xffffffffu, fp, j, kLanes);
         l += __shfl_sync(0xffffffffu, lp, j, kLanes);
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(
-            a.ws + (q0 + j ? 2 * (int64_t)(p0 + q0 + j) : w.slot(p0)) * kSlot + (int64_t)r * D + d));
-        acc.x += v.x * f;
-        acc.y += v.y * f;
-        acc.z += v.z * f;
-        acc.w += v.w * f;
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(q0 + j ? src + 2 * j * kSlot : first + at_acc));
+        acc[0] += v.x * f;
+        acc[1] += v.y * f;
+        acc[2] += v.z * f;
+        acc[3] += v.w * f;
       }
     }
-    const int row = w.tile * R + r;
-    if (r0 + lane / kLanes < rows)
-      finish_row<D, F16>(a, w.s.first + row / a.G, w.kvh * a.G + row % a.G, d, acc, top, l);
+    if (r0 + lane / kLanes < rows) finish_row<D, F16, 4>(a, w.token(a, r), w.head(a, r), d, acc, top, l);
   }
+}
+
+// Launch of the tcgen05 kernel (paged_prefill.cu): tiles of kTcRows rows.
+constexpr int kTcRows = 256;
+cudaError_t launch_paged_tc(int D, bool f16, const CUtensorMap& k, const CUtensorMap& v, const PagedArgs& a, int ctas,
+                            cudaStream_t s);
+
+// One box {64 dims, rows, one head, one page} of the pool into shared memory.
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int slot, int head, int page,
+                                         uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(slot), "r"(head), "r"(page), "r"(smem_addr(bar))
+      : "memory");
 }
 
 }  // namespace qi4

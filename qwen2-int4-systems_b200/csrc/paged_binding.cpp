@@ -201,7 +201,7 @@ at::Tensor attend(const at::Tensor& q, const at::Tensor& k_cache, const at::Tens
   }
   if (T == 0) return out;
   const c10::cuda::CUDAGuard guard(q.device());
-  const bool shared = prefix_length > 0;
+  const int64_t most = max_tokens ? *max_tokens : 0;
   at::Tensor ws;
   if (workspace) {
     ws = *workspace;
@@ -209,12 +209,12 @@ at::Tensor attend(const at::Tensor& q, const at::Tensor& k_cache, const at::Tens
     want(ws.is_cuda() && ws.get_device() == q.get_device() && ws.is_contiguous(),
          "workspace must be contiguous, on the tensors' device");
   } else {
-    ws = at::empty({static_cast<int64_t>(qi4_paged_attention_workspace(T, Hq, kv.head_dim, shared))},
-                   q.options().dtype(at::kByte));
+    const size_t bytes = qi4_paged_attention_workspace(T, Hq, kv.kv_heads, kv.head_dim, cu_tokens ? most : T / B,
+                                                       prefix_length > 0);
+    ws = at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte));
   }
   const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(q.get_device()).stream();
   const float sc = static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(q.size(2))));
-  const int64_t most = max_tokens ? *max_tokens : 0;
   const int rc =
       prefix_table
           ? qi4_shared_prefix_attention(&kv, q2.data_ptr(), q2.stride(0), q2.stride(1), out.data_ptr(), T, B, Hq,

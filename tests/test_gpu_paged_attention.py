@@ -85,7 +85,7 @@ def test_strided_queries_own_memory_and_streams(b200, cuda_device, tokens):
     joint = torch.randn(x["q"].shape[0], 12, 128, device=cuda_device).to(BF16)
     joint[:, :8] = x["q"]
     lib = importlib.import_module(b200.__name__ + "._lib").load()
-    n = lib.qi4_paged_attention_workspace(x["q"].shape[0], 8, 128, 0)
+    n = lib.qi4_paged_attention_workspace(x["q"].shape[0], 8, 2, 128, 0, 0)
     ws = torch.full((n,), 255, dtype=torch.uint8, device=cuda_device)
     out = torch.empty_like(x["q"])
     args = dict(cu_tokens=x["cu"], out=out, workspace=ws)
