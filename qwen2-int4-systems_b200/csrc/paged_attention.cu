@@ -18,7 +18,6 @@
 // the item's last unit, which is released afterwards.
 #include <algorithm>
 #include <atomic>
-#include <chrono>
 
 #include "paged_attention.cuh"
 
@@ -34,7 +33,7 @@ constexpr int stages_of(int D) { return D == 128 ? 3 : 6; }
 constexpr int stage_bytes(int D) { return 2 * kBlockKeys * D * 2; }
 constexpr size_t smem_of(int D, int NT) {
   return 1024 + (size_t)stages_of(D) * stage_bytes(D) + (size_t)8 * NT * (2 * D + 16) +
-         2 * 2 * kWarps * 8 * NT * sizeof(float) + 2 * stages_of(D) * sizeof(uint64_t) + 16;
+         2 * 2 * kWarps * 8 * NT * sizeof(float) + 2 * stages_of(D) * sizeof(uint64_t);
 }
 
 template <bool F16>
@@ -86,7 +85,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   float* red_l = red_m + 2 * kWarps * R;
   uint64_t* full = reinterpret_cast<uint64_t*>(red_l + 2 * kWarps * R);
   uint64_t* empty = full + kStages;
-  int* last_s = reinterpret_cast<int*>(empty + kStages);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -105,7 +103,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_launch_dependents();
 
   Walk<R> w;
-  if (!w.begin(a, lane)) return;
+  if (!w.begin(a, lane)) {
+    if (threadIdx.x == 0) note_split(a, w, false);
+    return;
+  }
   int stage = 0;
   uint32_t phase = 0;
 
@@ -158,22 +159,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   int par = 0;
   while (w.next(a)) {
     const int rows = w.rows(a), vis = w.tile_visible(a), nload = w.loaded(vis);
-    const int row0 = w.tile * R;
-    if (nload == 0 && !w.whole()) {
-      // A piece without visible keys still counts; its rows hold nothing.
-      float* slot = a.ws + (int64_t)w.slot(w.c) * (R * (D + 2));
-      for (int i = threadIdx.x; i < R * D / 4; i += 32 * kWarps)
-        reinterpret_cast<float4*>(slot)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int i = threadIdx.x; i < R; i += 32 * kWarps)
-        reinterpret_cast<float2*>(slot + R * D)[i] = make_float2(-INFINITY, 0.f);
-    } else if (nload == 0) {
+    if (nload == 0) {  // no row sees a key
       for (int i = threadIdx.x; i < rows * (D / 4); i += 32 * kWarps) {
         const int r = i / (D / 4);
         float none[4] = {0.f, 0.f, 0.f, 0.f};
         finish_row<D, F16, 4>(a, w.token(a, r), w.head(a, r), (i - r * (D / 4)) * 4, none, -INFINITY, 0.f);
       }
-    }
-    if (nload > 0) {
+    } else {
       // The tile's queries (rows past the last are zero).
       for (int i = threadIdx.x; i < R * (D / 8); i += 32 * kWarps) {
         const int r = i / (D / 8), ch = i - r * (D / 8);
@@ -198,7 +190,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int r = nt * 8 + 2 * tq + e;
-          lim[nt][e] = r < rows ? visible(a, w.s, row0 + r) : 0;
+          lim[nt][e] = r < rows ? w.row_visible(a, r) : 0;
           if (r < rows) lim_min = min(lim_min, lim[nt][e]);
         }
       lim_min = __reduce_min_sync(0xffffffffu, lim_min);
@@ -363,7 +355,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       constexpr int kLanes = D / 4;
       const bool whole = w.whole();
-      float* slot = whole ? nullptr : a.ws + (int64_t)w.slot(w.c) * (R * (D + 2));
+      float* slot = whole ? nullptr : a.ws + (int64_t)w.slot(blockIdx.x) * (R * (D + 2));
       for (int i = threadIdx.x; i < rows * kLanes; i += 32 * kWarps) {
         const int r = i / kLanes, d = (i - r * kLanes) * 4;
         float top = -INFINITY, sum = 0.f;
@@ -390,17 +382,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) mbar_arrive(&empty[held]);
       par ^= 1;
     }
-    if (!w.whole()) {
-      __threadfence();
-      named_barrier(1, 32 * kWarps);
-      if (threadIdx.x == 0) *last_s = arrive_last(a.counters + w.first_cta(), a.call, w.pieces());
-      named_barrier(1, 32 * kWarps);
-      if (*last_s) {
-        __threadfence();
-        merge_pieces<D, R, F16>(a, w, warp, kWarps, lane);
-      }
-    }
   }
+  if (threadIdx.x == 0) note_split(a, w, true);
 }
 
 }  // namespace
@@ -432,7 +415,8 @@ cudaError_t launch_decode(const CUtensorMap& k, const CUtensorMap& v, const Page
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, k, v, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, k, v, a);
+  return e != cudaSuccess ? e : launch_join<D, 8 * NT, F16>(a, ctas, s);
 }
 
 template <int D, bool F16>
@@ -454,24 +438,15 @@ constexpr int64_t kTcFrom = 65;
 bool takes_tc(int64_t tokens, int64_t G) { return tokens * G >= kTcFrom && G <= 128; }
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
-// Room for the pieces of a launch over `tokens` per sequence (and the counters).
+// Room for the pieces of a launch over `tokens` per sequence, and what the runs note of their split items.
 size_t pieces_bytes(int64_t tokens, int64_t G, int D, int ctas) {
   const size_t rows = takes_tc(tokens, G) ? kTcRows : 32;
-  return round256((size_t)ctas * (2 * rows * (D + 2) * sizeof(float) + 8));
+  return round256((size_t)ctas * (2 * rows * (D + 2) * sizeof(float) + sizeof(SplitItem)));
 }
 size_t state_bytes(int64_t T, int64_t Hq, int D) { return (size_t)(T * Hq) * (D + 2) * sizeof(float); }
 size_t workspace_bytes_for(int64_t T, int64_t Hq, int64_t Hkv, int D, int64_t most, bool prefix, int ctas) {
   return pieces_bytes(most, Hq / Hkv, D, ctas) +
          (prefix ? pieces_bytes(T, Hq / Hkv, D, ctas) + state_bytes(T, Hq, D) : 0);
-}
-
-// A number no other call of this process bears, and hardly one of another
-// process: the counters' words start from the clock.
-unsigned long long next_call() {
-  static std::atomic<unsigned long long> n{
-      (unsigned long long)std::chrono::steady_clock::now().time_since_epoch().count()};
-  const unsigned long long v = n.fetch_add(1, std::memory_order_relaxed) & ((1ull << 48) - 1);
-  return v ? v : 1;
 }
 
 struct Call {
@@ -521,8 +496,8 @@ int attend(const Call& c, const char* what) {
     return QI4_ERR_SHAPE;
   }
   auto al = [](const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
-  if (!al(c.q, 16) || !al(c.out, 16) || c.q_tok % 8 || c.q_head % 8 || c.q_tok < 0 || c.q_head < 0) {
-    set_error("%s: q and out must be 16-byte aligned, q with strides that are multiples of 8 elements", what);
+  if (!al(c.q, 16) || !al(c.out, 32) || c.q_tok % 8 || c.q_head % 8 || c.q_tok < 0 || c.q_head < 0) {
+    set_error("%s: q must be 16-byte and out 32-byte aligned, q with strides that are multiples of 8 elements", what);
     return QI4_ERR_ALIGNMENT;
   }
   const bool prefix = c.prefix_len > 0;
@@ -575,8 +550,7 @@ int attend(const Call& c, const char* what) {
     const bool tc = takes_tc(tokens, G);
     const size_t rows = tc ? kTcRows : 32;
     x.ws = reinterpret_cast<float*>(at);
-    x.counters = reinterpret_cast<unsigned long long*>(at + (size_t)sms * 2 * rows * (D + 2) * sizeof(float));
-    x.call = next_call();
+    x.splits = reinterpret_cast<SplitItem*>(at + (size_t)sms * 2 * rows * (D + 2) * sizeof(float));
     if (tc) return launch_paged_tc(D, f16, kmap, vmap, x, sms, c.stream);
     return launch_kernel(D, f16, tokens * G <= 8 ? 1 : tokens * G <= 16 ? 2 : 4, kmap, vmap, x, sms, c.stream);
   };

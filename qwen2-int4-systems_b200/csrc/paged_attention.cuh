@@ -1,19 +1,18 @@
 // Work split and partial-result merging of the paged attention kernels.
 //
-// A batch is cut into items - one row tile (R consecutive rows of one
+// A batch is cut into items - one row tile (up to R consecutive rows of one
 // sequence's tokens x the G query heads of one KV head, row = token * G + head)
-// of one KV head - and every item into units of kBlockKeys keys. The units of
-// all items, in one line, are dealt to the CTAs in equal runs, so sequences of
-// any mixture of lengths keep all SMs equally busy; a CTA's run may end inside
-// an item. An item wholly inside one run is finished there; the pieces of
-// another go to a workspace as (weighted sums, max, sum of weights) and the
-// CTA that delivers the last piece merges them all, in the order of the runs,
-// whoever it is: the result does not depend on the order of arrival.
-//
-// The pieces of an item are counted in a 64-bit word (call number << 16 |
-// pieces so far) that the merging CTA sets back to zero; a word that holds
-// another call's number counts as zero. So the workspace needs no
-// initialisation, and a captured graph may be replayed.
+// of one KV head - and every item into units of kBlockKeys keys that its rows
+// see. The units of all items, in one line, are dealt to the CTAs in equal
+// runs, so sequences of any mixture of lengths keep all SMs equally busy; a
+// CTA's run may end inside an item. An item wholly inside one run is finished there; the pieces of
+// another go to a workspace as (weighted sums, max, sum of weights), and a
+// second, small launch joins them in the order of the runs, so no result
+// depends on timing. (It is resident before the first launch ends, by
+// programmatic dependent launch. Counting the pieces in the kernel instead,
+// the last CTA of an item joining them, cost 25 us where 74 CTAs met at one
+// counter and one of them read all their pieces: 65 us for one sequence of
+// 131,002 keys against 32 with the second launch.)
 #pragma once
 
 #include "paged.cuh"
@@ -36,8 +35,7 @@ struct PagedArgs {
   int causal;
   float scale_log2;  // scale * log2(e)
   float* ws;         // pieces: two slots per CTA, each R x D sums then R x (max, sum)
-  unsigned long long* counters;  // one per CTA
-  unsigned long long call;       // number of this call, 1 .. 2^48 - 1
+  struct SplitItem* splits;  // one per CTA: the item that begins in its run and ends beyond it
   // Keys that every row has seen already (a shared prefix): per row t * Hq + h
   // the D weighted sums, and (max, sum of weights); or null.
   const float* prior_acc;
@@ -47,156 +45,165 @@ struct PagedArgs {
   float* state_ml;
 };
 
-struct Seq {
-  int first, n, len;  // first token row, tokens, keys
-  int tiles, blocks;  // row tiles, units of an item
-  __device__ __forceinline__ int units(int Hkv) const { return n > 0 ? tiles * Hkv * blocks : 0; }
+// An item whose pieces are joined: `pieces` of them (0: none), the first in
+// slot `slot`, piece p > 0 in slot 2 (cta + p). Row r of its tile is query row
+// row0 + r of the sequence whose first token is `first`.
+struct SplitItem {
+  int pieces, slot, rows, first, row0, kvh;
 };
-
-template <int R>
-__device__ __forceinline__ Seq seq_info(const PagedArgs& a, int b) {
-  const Tokens t = seq_tokens(a.r, b);
-  int len = a.fixed_len >= 0 ? a.fixed_len : __ldg(a.r.lengths + b);
-  len = min(max(len, 0), a.cap);
-  return {t.first, t.count, len, (t.count * a.G + R - 1) / R, max(1, (len + kBlockKeys - 1) / kBlockKeys)};
-}
-
-// Keys that row `row` of the sequence sees.
-__device__ __forceinline__ int visible(const PagedArgs& a, const Seq& s, int row) {
-  return a.causal ? max(0, min(s.len, s.len - s.n + row / a.G + 1)) : s.len;
-}
-
-// The units of all sequences: their number, and the sequence that holds unit
-// `u` with the units before it. Every lane of the warp takes part and gets
-// the same result; 128 sequences at a time, their loads independent.
-template <int R>
-__device__ __forceinline__ long long total_units(const PagedArgs& a, int lane) {
-  long long sum = 0;
-  for (int b0 = 0; b0 < a.r.B; b0 += 128) {
-    int w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int b = b0 + 4 * lane + i;
-      w[i] = b < a.r.B ? seq_info<R>(a, b).units(a.Hkv) : 0;
-    }
-    long long mine = (long long)w[0] + w[1] + w[2] + w[3];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    sum += mine;
-  }
-  return sum;
-}
-
-template <int R>
-__device__ __forceinline__ void find_unit(const PagedArgs& a, long long u, int lane, int& seq, long long& before) {
-  long long base = 0;
-  for (int b0 = 0; b0 < a.r.B; b0 += 128) {
-    int w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int b = b0 + 4 * lane + i;
-      w[i] = b < a.r.B ? seq_info<R>(a, b).units(a.Hkv) : 0;
-    }
-    const long long mine = (long long)w[0] + w[1] + w[2] + w[3];
-    long long incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
-    }
-    const long long all = __shfl_sync(0xffffffffu, incl, 31);
-    if (u < base + all) {
-      const unsigned hit = __ballot_sync(0xffffffffu, base + incl > u);
-      const int src = __ffs(hit) - 1;
-      long long at = base + incl - mine;
-      int s = 0;
-#pragma unroll
-      for (int i = 0; i < 3; ++i)
-        if (s == i && at + w[i] <= u) {
-          at += w[i];
-          ++s;
-        }
-      seq = __shfl_sync(0xffffffffu, b0 + 4 * lane + s, src);
-      before = __shfl_sync(0xffffffffu, at, src);
-      return;
-    }
-    base += all;
-  }
-  seq = a.r.B;
-  before = base;
-}
 
 // CTA c of C owns units [run_start(c), run_start(c + 1)); run_of inverts it.
 __device__ __forceinline__ long long run_start(int c, long long U, int C) { return (long long)c * U / C; }
 __device__ __forceinline__ int run_of(long long u, long long U, int C) { return (int)(((u + 1) * C + U - 1) / U) - 1; }
 
-// One CTA's walk over its units, item by item; every warp keeps its own copy.
+// One CTA's walk over its units, item by item; every warp keeps its own copy
+// (all lanes alike). A tile has R rows, or the most whole tokens that R rows
+// hold; an item has one unit per kBlockKeys keys that its last row sees, and
+// one more in front that stands for its fixed cost (queries, sums, output) in
+// the dealing and is no work: where a run ends behind it, the item begins
+// with the next CTA.
 template <int R>
 struct Walk {
-  long long U, u, end, item0;  // item0: first unit of the current item
-  int C, c, b, rem;            // rem: units of sequence b before u
-  Seq s;
-  int kvh, tile, blk, nblk;    // this piece: units [blk, blk + nblk) of the item
+  long long U, u, end, item0;  // u: next unit; item0: the current item's first (fixed-cost) unit
+  int C, tile_rows;
+  int b, first, n, len, tiles;       // sequence b: first token, tokens, keys, row tiles
+  int tile, kvh, blocks, at;         // item; at: next of its 1 + blocks units
+  int blk, nblk;                     // this piece: blocks [blk, blk + nblk) of the item
 
-  __device__ __forceinline__ bool begin(const PagedArgs& a, int lane) {
-    U = total_units<R>(a, lane);
-    C = (int)min((long long)gridDim.x, U);
-    c = blockIdx.x;
-    if (c >= C) return false;
-    u = run_start(c, U, C);
-    end = run_start(c + 1, U, C);
-    long long before;
-    find_unit<R>(a, u, lane, b, before);
-    rem = (int)(u - before);
-    s = seq_info<R>(a, min(b, a.r.B - 1));
-    return true;
+  __device__ __forceinline__ void load(const PagedArgs& a, int seq) {
+    b = seq;
+    const Tokens t = seq_tokens(a.r, seq);
+    first = t.first;
+    n = t.count;
+    len = a.fixed_len >= 0 ? a.fixed_len : __ldg(a.r.lengths + seq);
+    len = min(max(len, 0), a.cap);
+    tiles = (n * a.G + tile_rows - 1) / tile_rows;
   }
-  __device__ __forceinline__ bool next(const PagedArgs& a) {
-    if (u >= end) return false;
-    while (rem >= s.units(a.Hkv)) {
-      rem -= s.units(a.Hkv);
-      if (++b >= a.r.B) return false;
-      s = seq_info<R>(a, b);
+  // Keys that a row of the sequence sees.
+  __device__ __forceinline__ int visible(const PagedArgs& a, int seq_row) const {
+    return a.causal ? max(0, min(len, len - n + seq_row / a.G + 1)) : len;
+  }
+  __device__ __forceinline__ int blocks_of(const PagedArgs& a, int t) const {
+    return max(1, (visible(a, min(n * a.G, (t + 1) * tile_rows) - 1) + kBlockKeys - 1) / kBlockKeys);
+  }
+  // Units of sequences b0 .. b0 + per - 1, one per group of 32 / per lanes (per
+  // a power of two), each lane summing every (32 / per)-th tile; the sum of a
+  // sequence ends up in the first lane of its group, 0 in the others.
+  __device__ __forceinline__ long long group_units(const PagedArgs& a, int b0, int per, int lane) {
+    const int lanes = 32 / per, seq = b0 + lane / lanes, sub = lane % lanes;
+    long long sum = 0;
+    if (seq < a.r.B) {
+      load(a, seq);
+      if (!a.causal) {
+        if (sub == 0) sum = (long long)tiles * (1 + blocks_of(a, 0));
+      } else {
+        for (int t = sub; t < tiles; t += lanes) sum += 1 + blocks_of(a, t);
+      }
     }
-    const int item = rem / s.blocks;
-    blk = rem - item * s.blocks;
-    tile = item / a.Hkv;
-    kvh = item - tile * a.Hkv;
-    nblk = (int)min((long long)(s.blocks - blk), end - u);
-    item0 = u - blk;
-    u += nblk;
-    rem += nblk;
+    for (int o = lanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return sub == 0 ? sum * a.Hkv : 0;
+  }
+  static __device__ __forceinline__ long long scan(long long x, int lane) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += v;
+    }
+    return x;
+  }
+  // False if the CTA has no units.
+  __device__ __forceinline__ bool begin(const PagedArgs& a, int lane) {
+    tile_rows = a.G <= R ? R / a.G * a.G : R;
+    int per = 32;
+    while (per > 1 && per / 2 >= a.r.B) per >>= 1;
+    U = 0;
+    long long mine = 0;
+    for (int b0 = 0; b0 < a.r.B; b0 += per) {
+      long long x = mine = group_units(a, b0, per, lane);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+      U += x;
+    }
+    C = (int)min((long long)gridDim.x, U);
+    if ((int)blockIdx.x >= C) return false;
+    u = run_start(blockIdx.x, U, C);
+    end = run_start(blockIdx.x + 1, U, C);
+    // The sequence that holds unit u, then the tile.
+    long long before = 0;
+    int seq = 0;
+    for (int b0 = 0; b0 < a.r.B; b0 += per) {
+      if (a.r.B > per) mine = group_units(a, b0, per, lane);
+      const long long incl = scan(mine, lane);
+      const unsigned hit = __ballot_sync(0xffffffffu, before + incl > u);
+      if (hit) {
+        const int src = __ffs(hit) - 1;
+        seq = b0 + src / (32 / per);
+        before += __shfl_sync(0xffffffffu, incl - mine, src);
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    load(a, seq);
+    for (tile = 0; tile + 1 < tiles; tile += 32) {
+      const long long units = tile + lane < tiles ? (long long)(1 + blocks_of(a, tile + lane)) * a.Hkv : 0;
+      const long long incl = scan(units, lane);
+      const unsigned hit = __ballot_sync(0xffffffffu, before + incl > u);
+      if (hit) {
+        const int src = __ffs(hit) - 1;
+        tile += src;
+        before += __shfl_sync(0xffffffffu, incl - units, src);
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    blocks = blocks_of(a, tile);
+    at = (int)(u - before);
+    kvh = at / (1 + blocks);
+    at -= kvh * (1 + blocks);
     return true;
   }
-  __device__ __forceinline__ bool whole() const { return blk == 0 && nblk == s.blocks; }
-  __device__ __forceinline__ int rows(const PagedArgs& a) const { return min(R, s.n * a.G - tile * R); }
-  __device__ __forceinline__ int64_t token(const PagedArgs& a, int r) const { return s.first + (tile * R + r) / a.G; }
-  __device__ __forceinline__ int head(const PagedArgs& a, int r) const { return kvh * a.G + (tile * R + r) % a.G; }
+  // The next piece; false behind the last.
+  __device__ __forceinline__ bool next(const PagedArgs& a) {
+    for (;;) {
+      if (u >= end) return false;
+      if (at > blocks) {  // the next KV head, tile or sequence with tokens
+        at = 0;
+        if (++kvh == a.Hkv) {
+          kvh = 0;
+          if (++tile == tiles) {
+            tile = 0;
+            do {
+              if (b + 1 >= a.r.B) return false;
+              load(a, b + 1);
+            } while (tiles == 0);
+          }
+          blocks = blocks_of(a, tile);
+        }
+      }
+      const int take = (int)min((long long)(1 + blocks - at), end - u);
+      item0 = u - at;
+      blk = max(at - 1, 0);
+      nblk = at + take - 1 - blk;
+      u += take;
+      at += take;
+      if (nblk > 0) return true;
+    }
+  }
+  __device__ __forceinline__ bool whole() const { return nblk == blocks; }
+  __device__ __forceinline__ int rows(const PagedArgs& a) const { return min(tile_rows, n * a.G - tile * tile_rows); }
+  __device__ __forceinline__ int row0() const { return tile * tile_rows; }
+  __device__ __forceinline__ int64_t token(const PagedArgs& a, int r) const { return first + (row0() + r) / a.G; }
+  __device__ __forceinline__ int head(const PagedArgs& a, int r) const { return kvh * a.G + (row0() + r) % a.G; }
+  __device__ __forceinline__ int row_visible(const PagedArgs& a, int r) const { return visible(a, row0() + r); }
   // Keys the tile's last row sees: none beyond is loaded.
-  __device__ __forceinline__ int tile_visible(const PagedArgs& a) const {
-    return visible(a, s, tile * R + rows(a) - 1);
-  }
-  // Blocks of this piece that hold visible keys.
-  __device__ __forceinline__ int loaded(int vis) const {
-    return max(0, min(nblk, (vis + kBlockKeys - 1) / kBlockKeys - blk));
-  }
-  __device__ __forceinline__ int first_cta() const { return run_of(item0, U, C); }
-  __device__ __forceinline__ int pieces() const { return run_of(item0 + s.blocks - 1, U, C) - first_cta() + 1; }
-  // Where CTA p's piece of the current item lies: its first or its second slot.
+  __device__ __forceinline__ int tile_visible(const PagedArgs& a) const { return row_visible(a, rows(a) - 1); }
+  // Blocks of this piece that hold visible keys: all, but for an item of one empty block.
+  __device__ __forceinline__ int loaded(int vis) const { return vis > 0 ? nblk : 0; }
+  // The CTAs that hold the item's blocks, and where CTA p's piece lies: its first or its second slot.
+  __device__ __forceinline__ int first_cta() const { return run_of(item0 + 1, U, C); }
+  __device__ __forceinline__ int pieces() const { return run_of(item0 + blocks, U, C) - first_cta() + 1; }
   __device__ __forceinline__ int slot(int p) const { return 2 * p + (run_start(p, U, C) >= item0 ? 0 : 1); }
 };
-
-// Counts one piece of `n`; true for the piece that completes the item.
-__device__ __forceinline__ bool arrive_last(unsigned long long* word, unsigned long long call, int n) {
-  unsigned long long old = *reinterpret_cast<volatile unsigned long long*>(word);
-  for (;;) {
-    const int seen = (old >> 16) == call ? (int)(old & 0xFFFF) : 0;
-    const unsigned long long now = seen + 1 == n ? 0ull : (call << 16 | (unsigned)(seen + 1));
-    const unsigned long long got = atomicCAS(word, old, now);
-    if (got == old) return seen + 1 == n;
-    old = got;
-  }
-}
 
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
@@ -247,37 +254,59 @@ __device__ __forceinline__ void finish_row(const PagedArgs& a, int64_t token, in
   uint32_t w[N / 2];
 #pragma unroll
   for (int i = 0; i < N / 2; ++i) w[i] = pack2<F16>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
-  if constexpr (N == 8)
-    *reinterpret_cast<uint4*>(a.out + row * D + d) = make_uint4(w[0], w[1], w[2], w[3]);
+  uint16_t* out = a.out + row * D + d;
+  if constexpr (N == 16)  // one whole sector of 32 bytes
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
   else
-    *reinterpret_cast<uint2*>(a.out + row * D + d) = make_uint2(w[0], w[1]);
+    *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
 }
 
-// Merges the pieces of the walk's current item and finishes its rows: a group
-// of D / 4 lanes per row, warp `warp` of `nwarps`. Pieces in the order of
-// their CTAs: the first CTA's, then the first slot of each later one.
-template <int D, int R, bool F16, class W>
-__device__ __forceinline__ void merge_pieces(const PagedArgs& a, const W& w, int warp, int nwarps, int lane) {
+// What a CTA leaves for the joining launch, from its last piece (one thread).
+template <int R>
+__device__ __forceinline__ void note_split(const PagedArgs& a, const Walk<R>& w, bool any) {
+  SplitItem it = {0, 0, 0, 0, 0, 0};
+  if (any && w.blk == 0 && w.nblk > 0 && !w.whole())
+    it = {w.pieces(), w.slot(blockIdx.x), w.rows(a), w.first, w.row0(), w.kvh};
+  a.splits[blockIdx.x] = it;
+}
+
+// Joins the pieces of the item that begins in CTA blockIdx.x's run and ends
+// beyond it, if there is one: a group of D / 4 lanes per row, the rows spread
+// over the warps of the blocks (blockIdx.x, 0 ..).
+constexpr int kJoinThreads = 256;
+template <int D, int R, bool F16>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArgs a) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const SplitItem it = a.splits[blockIdx.x];
   constexpr int kLanes = D / 4, kPerWarp = 32 / kLanes;
   constexpr int64_t kSlot = (int64_t)R * (D + 2);
-  const int np = w.pieces(), p0 = w.first_cta(), rows = w.rows(a);
-  const float* first = a.ws + w.slot(p0) * kSlot;
-  const float* later = a.ws + 2 * (int64_t)p0 * kSlot;  // piece p > 0 at later + 2 p kSlot
-  const int d = (lane % kLanes) * 4;
-  for (int r0 = warp * kPerWarp; r0 < rows; r0 += nwarps * kPerWarp) {
-    const int r = min(r0 + lane / kLanes, rows - 1);
+  const int lane = threadIdx.x & 31, d = (lane % kLanes) * 4, np = it.pieces;
+  const float* first = a.ws + it.slot * kSlot;
+  const float* later = a.ws + 2 * (int64_t)blockIdx.x * kSlot;
+  for (int r0 = (blockIdx.y * (kJoinThreads / 32) + threadIdx.x / 32) * kPerWarp; r0 < it.rows;
+       r0 += gridDim.y * (kJoinThreads / 32) * kPerWarp) {
+    const int r = min(r0 + lane / kLanes, it.rows - 1);
     const int64_t at_ml = (int64_t)R * D + 2 * r, at_acc = (int64_t)r * D + d;
-    float top = -INFINITY;
-    for (int p = lane % kLanes; p < np; p += kLanes) top = fmaxf(top, __ldcg((p ? later + 2 * p * kSlot : first) + at_ml));
-#pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    float l = 0.f;
+    float top = -INFINITY, l = 0.f;
+    // 32 (16) pieces at a time, one lane each for their maxima and sums; the
+    // running maximum is moved once per round.
     for (int q0 = 0; q0 < np; q0 += kLanes) {
       const int p = q0 + lane % kLanes;
       float2 ml = make_float2(-INFINITY, 0.f);
-      if (p < np) ml = __ldcg(reinterpret_cast<const float2*>((p ? later + 2 * p * kSlot : first) + at_ml));
-      const float fp = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - top);
+      if (p < np) ml = *reinterpret_cast<const float2*>((p ? later + 2 * p * kSlot : first) + at_ml);
+      float m = fmaxf(top, ml.x);
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      const float back = top == -INFINITY ? 0.f : exp2_approx(top - m);
+      top = m;
+      l *= back;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] *= back;
+      const float fp = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - m);
       const float lp = ml.y * fp;
       const int cnt = min(kLanes, np - q0);
       const float* src = later + 2 * q0 * kSlot + at_acc;
@@ -285,15 +314,32 @@ __device__ __forceinline__ void merge_pieces(const PagedArgs& a, const W& w, int
       for (int j = 0; j < cnt; ++j) {
         const float f = __shfl_sync(0xffffffffu, fp, j, kLanes);
         l += __shfl_sync(0xffffffffu, lp, j, kLanes);
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(q0 + j ? src + 2 * j * kSlot : first + at_acc));
+        const float4 v = *reinterpret_cast<const float4*>(q0 + j ? src + 2 * j * kSlot : first + at_acc);
         acc[0] += v.x * f;
         acc[1] += v.y * f;
         acc[2] += v.z * f;
         acc[3] += v.w * f;
       }
     }
-    if (r0 + lane / kLanes < rows) finish_row<D, F16, 4>(a, w.token(a, r), w.head(a, r), d, acc, top, l);
+    if (r0 + lane / kLanes < it.rows)
+      finish_row<D, F16, 4>(a, it.first + (it.row0 + r) / a.G, it.kvh * a.G + (it.row0 + r) % a.G, d, acc, top, l);
   }
+}
+
+// Launches the joining of `ctas` runs, behind the kernel that wrote their pieces.
+template <int D, int R, bool F16>
+cudaError_t launch_join(const PagedArgs& a, int ctas, cudaStream_t s) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  constexpr int kRowsAtOnce = kJoinThreads / 32 * (128 / D);
+  cfg.gridDim = dim3((unsigned)ctas, (unsigned)((R + 2 * kRowsAtOnce - 1) / (2 * kRowsAtOnce)), 1);
+  cfg.blockDim = dim3(kJoinThreads, 1, 1);
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, paged_join_kernel<D, R, F16>, a);
 }
 
 // Launch of the tcgen05 kernel (paged_prefill.cu): tiles of kTcRows rows.

@@ -194,8 +194,8 @@ at::Tensor attend(const at::Tensor& q, const at::Tensor& k_cache, const at::Tens
   if (out_) {
     out = *out_;
     check_rows(out, T, k_cache, "out must have q's shape");
-    want(out.size(1) == Hq && out.is_contiguous() && (T == 0 || aligned16(out)),
-         "out must have q's shape, contiguous and 16-byte aligned");
+    want(out.size(1) == Hq && out.is_contiguous() && (T == 0 || reinterpret_cast<uintptr_t>(out.data_ptr()) % 32 == 0),
+         "out must have q's shape, contiguous and 32-byte aligned");
   } else {
     out = at::empty({T, Hq, q.size(2)}, q.options());
   }

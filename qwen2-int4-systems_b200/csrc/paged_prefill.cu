@@ -39,157 +39,14 @@ __device__ int g_paged_tc_error;
 
 namespace {
 
-constexpr int kThreads = 384;
+constexpr int kThreads = 320;
 constexpr int kSoftmaxWarps = 8;
-constexpr int kMergeRowBlocks = 16;
 constexpr int slot_bytes(int D) { return kBlockKeys * D * 2; }
 constexpr int ring_slots(int D) { return D == 128 ? 5 : 10; }
 constexpr size_t smem_of(int D) {
   return 1024 + (size_t)kTcRows * D * 2 + (size_t)ring_slots(D) * slot_bytes(D) +
-         (8 + 2 * ring_slots(D)) * sizeof(uint64_t) + 16;
+         (16 + 2 * ring_slots(D)) * sizeof(uint64_t) + 16;
 }
-
-// The walk of paged_attention.cuh over tiles of whole tokens, each item with
-// as many units as its last token sees.
-struct TileWalk {
-  long long U, u, end, item0;
-  int C, c, b, tile_tokens;
-  int first, n, len, tiles;          // sequence b
-  int tile, kvh, blocks, blk, nblk;  // this piece
-
-  __device__ __forceinline__ void load(const PagedArgs& a, int seq) {
-    b = seq;
-    const Tokens t = seq_tokens(a.r, seq);
-    first = t.first;
-    n = t.count;
-    len = a.fixed_len >= 0 ? a.fixed_len : __ldg(a.r.lengths + seq);
-    len = min(max(len, 0), a.cap);
-    tiles = (n + tile_tokens - 1) / tile_tokens;
-  }
-  __device__ __forceinline__ int visible(const PagedArgs& a, int token) const {
-    return a.causal ? max(0, min(len, len - n + token + 1)) : len;
-  }
-  __device__ __forceinline__ int blocks_of(const PagedArgs& a, int t) const {
-    return max(1, (visible(a, min(n, (t + 1) * tile_tokens) - 1) + kBlockKeys - 1) / kBlockKeys);
-  }
-  // Units of sequences b0 .. b0 + per - 1, one per group of 32 / per lanes (per
-  // a power of two), each lane summing every (32 / per)-th tile; the sum of a
-  // sequence ends up in the first lane of its group, 0 in the others.
-  __device__ __forceinline__ long long group_units(const PagedArgs& a, int b0, int per, int lane) {
-    const int lanes = 32 / per, seq = b0 + lane / lanes, sub = lane % lanes;
-    long long sum = 0;
-    if (seq < a.r.B) {
-      load(a, seq);
-      if (!a.causal) {
-        if (sub == 0) sum = (long long)tiles * blocks_of(a, 0);
-      } else {
-        for (int t = sub; t < tiles; t += lanes) sum += blocks_of(a, t);
-      }
-    }
-    for (int o = lanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    return sub == 0 ? sum * a.Hkv : 0;
-  }
-  __device__ __forceinline__ bool begin(const PagedArgs& a, int lane) {
-    tile_tokens = kTcRows / a.G;
-    int per = 32;
-    while (per > 1 && per / 2 >= a.r.B) per >>= 1;
-    U = 0;
-    for (int b0 = 0; b0 < a.r.B; b0 += per) {
-      long long x = group_units(a, b0, per, lane);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-      U += x;
-    }
-    C = (int)min((long long)gridDim.x, U);
-    c = blockIdx.x;
-    if (c >= C) return false;
-    u = run_start(c, U, C);
-    end = run_start(c + 1, U, C);
-    // The sequence that holds unit u, then the tile.
-    long long before = 0;
-    int seq = 0;
-    for (int b0 = 0; b0 < a.r.B; b0 += per) {
-      const long long mine = group_units(a, b0, per, lane);
-      long long incl = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += v;
-      }
-      const unsigned hit = __ballot_sync(0xffffffffu, before + incl > u);
-      if (hit) {
-        const int src = __ffs(hit) - 1;
-        seq = b0 + src / (32 / per);
-        before += __shfl_sync(0xffffffffu, incl - mine, src);
-        break;
-      }
-      before += __shfl_sync(0xffffffffu, incl, 31);
-    }
-    load(a, seq);
-    for (int t0 = 0;; t0 += 32) {
-      const long long mine = t0 + lane < tiles ? (long long)blocks_of(a, t0 + lane) * a.Hkv : 0;
-      long long incl = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += v;
-      }
-      const unsigned hit = __ballot_sync(0xffffffffu, before + incl > u);
-      if (hit || t0 + 32 >= tiles) {
-        const int src = hit ? __ffs(hit) - 1 : 31;
-        tile = t0 + src;
-        before += __shfl_sync(0xffffffffu, incl - mine, src);
-        break;
-      }
-      before += __shfl_sync(0xffffffffu, incl, 31);
-    }
-    blocks = blocks_of(a, tile);
-    const int rem = (int)(u - before);
-    kvh = rem / blocks;
-    blk = rem - kvh * blocks;
-    nblk = 0;
-    return true;
-  }
-  __device__ __forceinline__ bool next(const PagedArgs& a) {
-    if (u >= end) return false;
-    blk += nblk;
-    if (blk >= blocks) {  // the next KV head, tile or sequence with tokens
-      blk = 0;
-      if (++kvh == a.Hkv) {
-        kvh = 0;
-        if (++tile == tiles) {
-          tile = 0;
-          do {
-            if (b + 1 >= a.r.B) return false;
-            load(a, b + 1);
-          } while (tiles == 0);
-        }
-        blocks = blocks_of(a, tile);
-      }
-    }
-    nblk = (int)min((long long)(blocks - blk), end - u);
-    item0 = u - blk;
-    u += nblk;
-    return true;
-  }
-  __device__ __forceinline__ bool whole() const { return blk == 0 && nblk == blocks; }
-  __device__ __forceinline__ int rows(const PagedArgs& a) const {
-    return min(tile_tokens, n - tile * tile_tokens) * a.G;
-  }
-  __device__ __forceinline__ int64_t token(const PagedArgs& a, int r) const {
-    return first + tile * tile_tokens + r / a.G;
-  }
-  __device__ __forceinline__ int head(const PagedArgs& a, int r) const { return kvh * a.G + r % a.G; }
-  __device__ __forceinline__ int row_visible(const PagedArgs& a, int r) const {
-    return visible(a, tile * tile_tokens + r / a.G);
-  }
-  __device__ __forceinline__ int tile_visible(const PagedArgs& a) const {
-    return visible(a, min(n, (tile + 1) * tile_tokens) - 1);
-  }
-  __device__ __forceinline__ int first_cta() const { return run_of(item0, U, C); }
-  __device__ __forceinline__ int pieces() const { return run_of(item0 + blocks - 1, U, C) - first_cta() + 1; }
-  __device__ __forceinline__ int slot(int p) const { return 2 * p + (run_start(p, U, C) >= item0 ? 0 : 1); }
-};
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
@@ -228,6 +85,13 @@ __device__ __forceinline__ void tmem_ld(uint32_t taddr, float* r) {
         "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
       : "r"(taddr));
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]),
+        "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
+      : "r"(taddr));
+}
 // Waits for the loads, and keeps every use of the N values behind the wait.
 template <int N>
 __device__ __forceinline__ void tmem_ld_wait(float* r) {
@@ -235,7 +99,14 @@ __device__ __forceinline__ void tmem_ld_wait(float* r) {
 #pragma unroll
   for (int i = 0; i < N; ++i) asm volatile("" : "+f"(r[i]));
 }
-// 16 or 32 columns of 32-bit words.
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
@@ -277,9 +148,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* q_s = smem;                      // 2 tiles [D / 64][128 rows][128 B]
   uint8_t* ring = smem + 2 * kTileBytes;    // slots [D / 64][128 keys][128 B]
   uint64_t* q_full = reinterpret_cast<uint64_t*>(ring + kSlots * kSlotBytes);  // [2] 4 warps
-  uint64_t* s_full = q_full + 2;                                               // [2] commit
-  uint64_t* p_full = s_full + 2;                                               // [2] 4 warps
-  uint64_t* o_full = p_full + 2;                                               // [2] commit
+  uint64_t* s_full = q_full + 2;                                               // [2 tiles][2 halves] commit
+  uint64_t* p_full = s_full + 4;                                               // [2][2] 4 warps
+  uint64_t* o_done = p_full + 4;                                               // [2] commit, per half
+  uint64_t* o_full = o_done + 2;                                               // [2] commit, per item
   uint64_t* kv_full = o_full + 2;                                              // [kSlots] TMA
   uint64_t* kv_empty = kv_full + kSlots;                                       // [kSlots] commit
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kv_empty + kSlots);
@@ -288,9 +160,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 4);
+      mbar_init(&o_done[i], 1);
+      mbar_init(&o_full[i], 1);
+    }
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
-      mbar_init(&o_full[i], 1);
     }
     for (int i = 0; i < kSlots; ++i) {
       mbar_init(&kv_full[i], 1);
@@ -308,7 +183,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_wait();
   pdl_launch_dependents();
 
-  TileWalk w;
+  Walk<kTcRows> w;
   const bool any = w.begin(a, lane);
   if (any && warp == kSoftmaxWarps + 1) {
     // ---- producer ----
@@ -347,57 +222,69 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (any && warp == kSoftmaxWarps) {
     // ---- products ----
-    if (lane == 0) {
-      constexpr uint32_t s_id = idesc(F16, kBlockKeys, false), o_id = idesc(F16, D, true);
-      int pos = 0;
-      uint32_t nq[2] = {0, 0}, np[2] = {0, 0};
-      auto scores = [&](int t, int st) {
-        const uint32_t qa = smem_addr(q_s + t * kTileBytes), ka = smem_addr(ring + st * kSlotBytes);
+    // The whole warp runs the loops and the waits; one lane issues.
+    constexpr uint32_t s_id = idesc(F16, 64, false), o_id = idesc(F16, D, true);
+    const uint64_t q_desc = sw128_desc(smem_addr(q_s)), k_desc = sw128_desc(smem_addr(ring)),
+                   v_desc0 = v_desc<D>(smem_addr(ring));  // (descriptors count addresses in 16 bytes)
+    int pos = 0;
+    uint32_t nq[2] = {0, 0}, np[2] = {0, 0};  // uses of q_full, and of p_full of either half
+    // Scores of tile t and the keys of half x of slot st; frees the slot behind the last.
+    auto scores = [&](int t, int x, int st, bool last) {
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t qd = q_desc + t * (kTileBytes >> 4), kd = k_desc + (st * kSlotBytes + x * 64 * 128) / 16;
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-          tc_mma(tmem + 128 * t, sw128_desc(qa + (k / 4) * kHalf + (k % 4) * 32),
-                 sw128_desc(ka + (k / 4) * kHalf + (k % 4) * 32), s_id, k > 0);
-        tc_commit(&s_full[t]);
-      };
-      while (w.next(a)) {
-        const int vis = w.tile_visible(a);
-        const int nload = max(0, min(w.nblk, (vis + kBlockKeys - 1) / kBlockKeys - w.blk));
-        if (nload == 0) continue;
-        const int nt = w.rows(a) > 128 ? 2 : 1;
-        int st = pos % kSlots;
-        mbar_wait(&kv_full[st], (uint32_t)(pos / kSlots) & 1u, &g_paged_tc_error);
-        for (int t = 0; t < nt; ++t) {
-          mbar_wait(&q_full[t], nq[t]++ & 1u, &g_paged_tc_error);
-          tc_fence_after();
-          scores(t, st);
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t at = ((k / 4) * kHalf + (k % 4) * 32) >> 4;
+          tc_mma(tmem + 128 * t + 64 * x, qd + at, kd + at, s_id, k > 0);
         }
-        tc_commit(&kv_empty[st]);
-        ++pos;
-        for (int i = 0; i < nload; ++i) {
-          const int vs = pos % kSlots, ks = (pos + 1) % kSlots;
-          for (int t = 0; t < nt; ++t) {
-            mbar_wait(&p_full[t], np[t]++ & 1u, &g_paged_tc_error);
-            if (t == 0) mbar_wait(&kv_full[vs], (uint32_t)(pos / kSlots) & 1u, &g_paged_tc_error);
-            tc_fence_after();
-            const uint32_t va = smem_addr(ring + vs * kSlotBytes);
+        tc_commit(&s_full[2 * t + x]);
+        if (last) tc_commit(&kv_empty[st]);
+      }
+      __syncwarp();
+    };
+    while (w.next(a)) {
+      const int nload = w.loaded(w.tile_visible(a));
+      if (nload == 0) continue;
+      const int nt = w.rows(a) > 128 ? 2 : 1;
+      const int k0 = pos % kSlots;
+      mbar_wait(&kv_full[k0], (uint32_t)(pos / kSlots) & 1u, &g_paged_tc_error);
+      for (int t = 0; t < nt; ++t) {
+        mbar_wait(&q_full[t], nq[t]++ & 1u, &g_paged_tc_error);
+        scores(t, 0, k0, false);
+      }
+      for (int t = 0; t < nt; ++t) scores(t, 1, k0, t == nt - 1);
+      ++pos;
+      for (int i = 0; i < nload; ++i) {
+        const bool more = i + 1 < nload;
+        const int vs = pos % kSlots, ks = (pos + 1) % kSlots;
 #pragma unroll
-            for (int k = 0; k < kBlockKeys / 16; ++k)
-              tc_mma_ta(tmem + 256 + D * t, tmem + 128 * t + 8 * k, v_desc<D>(va + k * 2048), o_id, i > 0 || k > 0);
-            if (t == nt - 1) tc_commit(&kv_empty[vs]);
-            if (i + 1 < nload) {
-              if (t == 0) mbar_wait(&kv_full[ks], (uint32_t)((pos + 1) / kSlots) & 1u, &g_paged_tc_error);
-              tc_fence_after();
-              scores(t, ks);
-              if (t == nt - 1) tc_commit(&kv_empty[ks]);
-            } else {
-              tc_commit(&o_full[t]);
+        for (int x = 0; x < 2; ++x)
+          for (int t = 0; t < nt; ++t) {
+            mbar_wait(&p_full[2 * t + x], np[t] & 1u, &g_paged_tc_error);
+            if (x == 0 && t == 0) mbar_wait(&kv_full[vs], (uint32_t)(pos / kSlots) & 1u, &g_paged_tc_error);
+            tc_fence_after();
+            if (elect_one()) {
+              const uint64_t vd = v_desc0 + vs * (kSlotBytes >> 4);
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                tc_mma_ta(tmem + 256 + D * t, tmem + 128 * t + 64 * x + 8 * k, vd + (4 * x + k) * (2048 >> 4), o_id,
+                          i > 0 || x > 0 || k > 0);
+              tc_commit(&o_done[t]);
+              if (x == 1 && !more) tc_commit(&o_full[t]);
+              if (x == 1 && t == nt - 1) tc_commit(&kv_empty[vs]);
+            }
+            __syncwarp();
+            if (x == 1) ++np[t];
+            if (more) {
+              if (x == 0 && t == 0) mbar_wait(&kv_full[ks], (uint32_t)((pos + 1) / kSlots) & 1u, &g_paged_tc_error);
+              scores(t, x, ks, x == 1 && t == nt - 1);
             }
           }
-          pos += i + 1 < nload ? 2 : 1;
-        }
+        pos += more ? 2 : 1;
       }
     }
-  } else if (any && warp < kSoftmaxWarps) {
+  } else if (warp < kSoftmaxWarps) {
     // ---- softmax, queries, epilogue ----
     const int t = warp >> 2, r = (warp & 3) * 32 + lane;  // row r of tile t
     const int row = t * 128 + r;
@@ -407,144 +294,162 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t sign = a.scale_log2 < 0.f ? 0x80008000u : 0u;
     const float scale = fmaxf(fabsf(a.scale_log2), 1e-30f);
     int pos = 0;
-    uint32_t ns = 0, no = 0;
-    while (w.next(a)) {
-      const int rows = w.rows(a), vis = w.tile_visible(a);
-      const int nload = max(0, min(w.nblk, (vis + kBlockKeys - 1) / kBlockKeys - w.blk));
+    uint32_t ns = 0, no = 0, done = 0;  // uses of s_full (of either half), o_full, and o_done
+    // The queries of the walk's item into this tile's shared memory, 16-byte chunks, rows past the last zero.
+    auto queries = [&]() {
+      const int rows = w.rows(a);
+      if (t * 128 >= rows || w.loaded(w.tile_visible(a)) == 0) return;
+      constexpr int kStep = 128 / (D / 8);  // rows between a thread's chunks
+      const int ch = threadIdx.x % (D / 8), r1 = (threadIdx.x % 128) / (D / 8);
+      const uint32_t dst = smem_addr(q_s + t * kTileBytes) + (ch >> 3) * kHalf;
+#pragma unroll
+      for (int g = 0; g < 128 / kStep; g += 8) {
+        uint4 v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int x = t * 128 + r1 + (g + i) * kStep;
+          v[i] = make_uint4(0u, 0u, 0u, 0u);
+          if (x < rows)
+            v[i] = *reinterpret_cast<const uint4*>(a.q + w.token(a, x) * a.q_tok + w.head(a, x) * a.q_head + ch * 8);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int qr = r1 + (g + i) * kStep;
+          sts128(dst + qr * 128 + (((ch & 7) ^ (qr & 7)) << 4),
+                 make_uint4(v[i].x ^ sign, v[i].y ^ sign, v[i].z ^ sign, v[i].w ^ sign));
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full[t]);
+    };
+    bool have = any && w.next(a);
+    if (have) queries();
+    while (have) {
+      const int rows = w.rows(a), vis = w.tile_visible(a), nload = w.loaded(vis);
       const int base_pos = pos;
       pos += 2 * nload;
-      if (t * 128 >= rows) continue;
-      const bool whole = w.whole();
-      float* slot = whole ? nullptr : a.ws + (int64_t)w.slot(w.c) * (kTcRows * (D + 2));
+      if (t * 128 >= rows) {
+        have = w.next(a);
+        if (have) queries();
+        continue;
+      }
+      const bool whole = w.whole(), live = row < rows;
+      float* slot = whole ? nullptr : a.ws + (int64_t)w.slot(blockIdx.x) * (kTcRows * (D + 2));
+      const int token = live ? (int)w.token(a, row) : 0, head = live ? w.head(a, row) : 0;
+      const int lim = live ? w.row_visible(a, row) : 0, blk0 = w.blk;
       float m = -INFINITY, l = 0.f;
-      if (nload > 0) {
-        // The queries of this tile: 16-byte chunks, rows past the last zero.
-        for (int i = (warp & 3) * 32 + lane; i < 128 * (D / 8); i += 128) {
-          const int qr = i / (D / 8), ch = i - qr * (D / 8), x = t * 128 + qr;
-          uint4 v = make_uint4(0u, 0u, 0u, 0u);
-          if (x < rows) {
-            v = *reinterpret_cast<const uint4*>(a.q + w.token(a, x) * a.q_tok + w.head(a, x) * a.q_head + ch * 8);
-            v.x ^= sign, v.y ^= sign, v.z ^= sign, v.w ^= sign;
-          }
-          sts128(smem_addr(q_s + t * kTileBytes) + (ch >> 3) * kHalf + qr * 128 + (((ch & 7) ^ (qr & 7)) << 4), v);
+      for (int h = 0; h < 2 * nload; ++h) {  // halves of 64 keys
+        const int x = h & 1, key0 = (blk0 + (h >> 1)) * kBlockKeys + 64 * x;
+        const uint32_t s_at = s_tm + 64 * x;
+        mbar_wait(&s_full[2 * t + x], ns & 1u, &g_paged_tc_error);
+        ns += x;
+        tc_fence_after();
+        float s[64];
+        tmem_ld(s_at, s);
+        tmem_ld(s_at + 32, s + 32);
+        tmem_ld_wait<64>(s);
+        if (__any_sync(0xffffffffu, lim < key0 + 64)) {
+#pragma unroll
+          for (int k = 0; k < 64; ++k) s[k] = key0 + k < lim ? s[k] : -INFINITY;
         }
-        fence_proxy_async_smem();
+        float mx[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mx[j] = fmaxf(s[j], s[j + 4]);
+#pragma unroll
+        for (int k = 8; k < 64; k += 8)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) mx[j] = max3(mx[j], s[k + j], s[k + 4 + j]);
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+        const bool move = top > m + 8.f;
+        if (__any_sync(0xffffffffu, move)) {
+          const float to = move ? top : m;
+          if (h > 0) {
+            // The sums of the half before must be complete (phase done + h - 1); those of the halves before it are,
+            // as the scores just read were issued behind them, so the phase's parity says which one it is.
+            mbar_wait(&o_done[t], (done + h - 1) & 1u, &g_paged_tc_error);
+            tc_fence_after();
+            const float f = move ? exp2_approx(m - to) : 1.f;
+            l *= f;
+#pragma unroll 1
+            for (int c = 0; c < D / 16; ++c) {
+              float o[16];
+              tmem_ld16(o_tm + 16 * c, o);
+              tmem_ld_wait<16>(o);
+#pragma unroll
+              for (int k = 0; k < 16; ++k) o[k] *= f;
+              tmem_st16(o_tm + 16 * c, reinterpret_cast<uint32_t*>(o));
+            }
+          }
+          m = to;
+        }
+        const float nb = m == -INFINITY ? 0.f : -m;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t p[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            float &u = s[32 * c + 2 * k], &v = s[32 * c + 2 * k + 1];
+            fma_pair(u, v, scale, nb);
+            u = exp2_approx(u);
+            v = exp2_approx(v);
+            add_pair(sum[(k & 1) * 2], sum[(k & 1) * 2 + 1], u, v);
+            p[k] = pack2<F16>(u, v);
+          }
+          tmem_st16(s_at + 16 * c, p);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        if (t == 0 && x == 0 && key0 + kBlockKeys > vis) {
+          // Slots past the last key may hold anything: their values are zeroed, as a weight of zero times a NaN is
+          // not zero.
+          const int vp = base_pos + h + 1, st = vp % kSlots;
+          mbar_wait(&kv_full[st], (uint32_t)(vp / kSlots) & 1u, &g_paged_tc_error);
+          if (key0 + r >= vis) {
+            const uint32_t at = smem_addr(ring + st * kSlotBytes) + r * 128;
+#pragma unroll
+            for (int k = 0; k < D / 8; ++k) sts128(at + (k >> 3) * kHalf + (k & 7) * 16, make_uint4(0u, 0u, 0u, 0u));
+          }
+          fence_proxy_async_smem();
+        }
+        tmem_st_wait();
+        tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&q_full[t]);
-        const int lim = row < rows ? w.row_visible(a, row) : 0;
-        for (int i = 0; i < nload; ++i) {
-          const int key0 = (w.blk + i) * kBlockKeys;
-          mbar_wait(&s_full[t], ns++ & 1u, &g_paged_tc_error);
-          tc_fence_after();
-          float s[128];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld(s_tm + 32 * c, s + 32 * c);
-          tmem_ld_wait<128>(s);
-          if (__any_sync(0xffffffffu, lim < key0 + kBlockKeys)) {
-#pragma unroll
-            for (int k = 0; k < 128; ++k) s[k] = key0 + k < lim ? s[k] : -INFINITY;
-          }
-          float mx[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) mx[k] = s[k];
-#pragma unroll
-          for (int k = 4; k < 128; k += 8) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              mx[j] = k + 4 + j < 128 ? max3(mx[j], s[k + j], s[k + 4 + j]) : fmaxf(mx[j], s[k + j]);
-          }
-          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
-          const bool move = top > m + 8.f || (m == -INFINITY && top > m);
-          if (__any_sync(0xffffffffu, move)) {
-            const float to = move ? top : m;
-            if (i > 0) {
-              const float f = move ? exp2_approx(m - to) : 1.f;
-              l *= f;
-#pragma unroll
-              for (int c = 0; c < D / 32; ++c) {
-                float o[32];
-                tmem_ld(o_tm + 32 * c, o);
-                tmem_ld_wait<32>(o);
-                uint32_t x[32];
-#pragma unroll
-                for (int k = 0; k < 32; ++k) x[k] = __float_as_uint(o[k] * f);
-                tmem_st32(o_tm + 32 * c, x);
-              }
-              tmem_st_wait();
-            }
-            m = to;
-          }
-          const float nb = m == -INFINITY ? 0.f : -m;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t p[32];
-#pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              float& x = s[64 * c + 2 * k];
-              float& y = s[64 * c + 2 * k + 1];
-              fma_pair(x, y, scale, nb);
-              x = exp2_approx(x);
-              y = exp2_approx(y);
-              add_pair(sum[(k & 1) * 2], sum[(k & 1) * 2 + 1], x, y);
-              p[k] = pack2<F16>(x, y);
-            }
-            tmem_st32(s_tm + 32 * c, p);
-          }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-          if (t == 0 && key0 + kBlockKeys > vis) {
-            // Slots past the last key may hold anything: their values are zeroed, as a weight of zero times a NaN
-            // is not zero.
-            const int vp = base_pos + 2 * i + 1, st = vp % kSlots;
-            mbar_wait(&kv_full[st], (uint32_t)(vp / kSlots) & 1u, &g_paged_tc_error);
-            if (key0 + r >= vis) {
-              const uint32_t at = smem_addr(ring + st * kSlotBytes) + r * 128;
-#pragma unroll
-              for (int x = 0; x < D / 8; ++x) sts128(at + (x >> 3) * kHalf + (x & 7) * 16, make_uint4(0u, 0u, 0u, 0u));
-            }
-            fence_proxy_async_smem();
-          }
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[t]);
-        }
+        if (lane == 0) mbar_arrive(&p_full[2 * t + x]);
+      }
+      // All scores of this item have been read, so the next one's queries may replace its own; the products go on
+      // with it while the sums of this one are written out.
+      have = w.next(a);
+      if (have) queries();
+      if (nload > 0) {
+        done += 2 * nload;
         mbar_wait(&o_full[t], no++ & 1u, &g_paged_tc_error);
         tc_fence_after();
       }
-      // ---- the rows' sums: out, or a piece ----
-      const bool live = row < rows;
-      const int64_t token = live ? w.token(a, row) : 0;
-      const int head = live ? w.head(a, row) : 0;
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        float o[32];
+      for (int c = 0; c < D / 16; ++c) {
+        float o[16];
         if (nload > 0) {
-          tmem_ld(o_tm + 32 * c, o);
-          tmem_ld_wait<32>(o);
+          tmem_ld16(o_tm + 16 * c, o);
+          tmem_ld_wait<16>(o);
         } else {
 #pragma unroll
-          for (int k = 0; k < 32; ++k) o[k] = 0.f;
+          for (int k = 0; k < 16; ++k) o[k] = 0.f;
         }
         if (live) {
+          if (whole) {
+            finish_row<D, F16, 16>(a, token, head, 16 * c, o, m, l);
+          } else {
+            float4* to = reinterpret_cast<float4*>(slot + row * D + 16 * c);
 #pragma unroll
-          for (int k = 0; k < 32; k += 8) {
-            float x[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = o[k + j];
-            if (whole) {
-              finish_row<D, F16, 8>(a, token, head, 32 * c + k, x, m, l);
-            } else {
-              float4* at = reinterpret_cast<float4*>(slot + row * D + 32 * c + k);
-              at[0] = make_float4(x[0], x[1], x[2], x[3]);
-              at[1] = make_float4(x[4], x[5], x[6], x[7]);
-            }
+            for (int k = 0; k < 4; ++k) to[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
           }
         }
       }
       if (live && !whole) *reinterpret_cast<float2*>(slot + kTcRows * D + 2 * row) = make_float2(m, l);
-      tc_fence_before();  // the sums are read before the next item's first product (behind q_full and p_full)
+      tc_fence_before();  // the sums are read before the next item's first weights are announced
     }
+    if (threadIdx.x == 0) note_split(a, w, any);
   }
   tc_fence_before();
   __syncthreads();
@@ -553,20 +458,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
-}
-
-// Joins the pieces of split items: block (c, y) takes every 16th group of rows
-// of the item that begins in CTA c's run and ends beyond it, if there is one.
-template <int D, bool F16>
-__global__ void __launch_bounds__(256) paged_merge_kernel(const PagedArgs a) {
-  pdl_wait();
-  pdl_launch_dependents();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  TileWalk w;
-  if (!w.begin(a, lane)) return;
-  bool found = false;
-  while (w.next(a)) found = w.blk == 0 && w.nblk < w.blocks;
-  if (found) merge_pieces<D, kTcRows, F16>(a, w, warp + 8 * blockIdx.y, 8 * gridDim.y, lane);
 }
 
 template <int D, bool F16>
@@ -592,11 +483,7 @@ cudaError_t launch(const CUtensorMap& k, const CUtensorMap& v, const PagedArgs& 
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, k, v, a);
-  if (e != cudaSuccess) return e;
-  cfg.gridDim = dim3((unsigned)ctas, kMergeRowBlocks, 1);
-  cfg.blockDim = dim3(256, 1, 1);
-  cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, paged_merge_kernel<D, F16>, a);
+  return e != cudaSuccess ? e : launch_join<D, kTcRows, F16>(a, ctas, s);
 }
 
 }  // namespace
