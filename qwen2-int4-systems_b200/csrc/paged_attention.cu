@@ -163,15 +163,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = threadIdx.x; i < rows * (D / 4); i += 32 * kWarps) {
         const int r = i / (D / 4);
         float none[4] = {0.f, 0.f, 0.f, 0.f};
-        finish_row<D, F16, 4>(a, w.token(a, r), w.head(a, r), (i - r * (D / 4)) * 4, none, -INFINITY, 0.f);
+        int token, head;
+        w.place(a, r, token, head);
+        finish_row<D, F16, 4>(a, token, head, (i - r * (D / 4)) * 4, none, -INFINITY, 0.f);
       }
     } else {
       // The tile's queries (rows past the last are zero).
       for (int i = threadIdx.x; i < R * (D / 8); i += 32 * kWarps) {
         const int r = i / (D / 8), ch = i - r * (D / 8);
         uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (r < rows)
-          v = *reinterpret_cast<const uint4*>(a.q + w.token(a, r) * a.q_tok + w.head(a, r) * a.q_head + ch * 8);
+        if (r < rows) {
+          int token, head;
+          w.place(a, r, token, head);
+          v = *reinterpret_cast<const uint4*>(a.q + token * a.q_tok + head * a.q_head + ch * 8);
+        }
         sts128(smem_addr(q_s) + r * kQRow + ch * 16, v);
       }
       named_barrier(1, 32 * kWarps);
@@ -371,7 +376,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           acc[0] += v.x, acc[1] += v.y, acc[2] += v.z, acc[3] += v.w;
         }
         if (whole) {
-          finish_row<D, F16, 4>(a, w.token(a, r), w.head(a, r), d, acc, top, sum);
+          int token, head;
+          w.place(a, r, token, head);
+          finish_row<D, F16, 4>(a, token, head, d, acc, top, sum);
         } else {
           *reinterpret_cast<float4*>(slot + r * D + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
           if (d == 0) *reinterpret_cast<float2*>(slot + R * D + 2 * r) = make_float2(top, sum);
@@ -384,6 +391,89 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
   if (threadIdx.x == 0) note_split(a, w, true);
+}
+
+// Joins the pieces of the item that begins in CTA blockIdx.x's run and ends
+// beyond it, if there is one; a block for each row. Groups of D / 4 lanes take
+// the pieces by turns, up to eight at once (one round of loads for 64 or 128
+// pieces), then their sums meet in shared memory in the groups' order.
+constexpr int kJoinThreads = 256;
+template <int D, int R, bool F16>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArgs a) {
+  constexpr int kLanes = D / 4, kGroups = kJoinThreads / kLanes, kAtOnce = 8;
+  constexpr int64_t kSlot = (int64_t)R * (D + 2);
+  __shared__ float4 acc_s[kGroups][kLanes];
+  __shared__ float2 ml_s[kGroups];
+  pdl_wait();
+  pdl_launch_dependents();
+  const SplitItem it = a.splits[blockIdx.x];
+  const int r = blockIdx.y, np = it.pieces;
+  if (r >= it.rows) return;
+  const int group = threadIdx.x / kLanes, d = (threadIdx.x % kLanes) * 4;
+  const float* first = a.ws + it.slot * kSlot;
+  const float* later = a.ws + 2 * (int64_t)blockIdx.x * kSlot;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float top = -INFINITY, l = 0.f;
+  for (int q0 = group; q0 < np; q0 += kGroups * kAtOnce) {
+    float2 ml[kAtOnce];
+    float4 v[kAtOnce];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      const int p = q0 + j * kGroups;
+      ml[j] = make_float2(-INFINITY, 0.f);
+      v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (p < np) {
+        const float* src = p ? later + 2 * p * kSlot : first;
+        ml[j] = *reinterpret_cast<const float2*>(src + R * D + 2 * r);
+        v[j] = *reinterpret_cast<const float4*>(src + r * D + d);
+      }
+    }
+    float to = top;
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) to = fmaxf(to, ml[j].x);
+    const float base = to == -INFINITY ? 0.f : to, back = exp2_approx(top - base);
+    top = to;
+    l *= back;
+    acc = make_float4(acc.x * back, acc.y * back, acc.z * back, acc.w * back);
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      const float f = exp2_approx(ml[j].x - base);
+      l += ml[j].y * f;
+      acc = make_float4(acc.x + v[j].x * f, acc.y + v[j].y * f, acc.z + v[j].z * f, acc.w + v[j].w * f);
+    }
+  }
+  acc_s[group][threadIdx.x % kLanes] = acc;
+  if (d == 0) ml_s[group] = make_float2(top, l);
+  __syncthreads();
+  if (group == 0) {
+    float to = -INFINITY, sum = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) to = fmaxf(to, ml_s[g].x);
+    const float base = to == -INFINITY ? 0.f : to;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      const float f = exp2_approx(ml_s[g].x - base);
+      const float4 v = acc_s[g][threadIdx.x];
+      sum += ml_s[g].y * f;
+      x[0] += v.x * f, x[1] += v.y * f, x[2] += v.z * f, x[3] += v.w * f;
+    }
+    const int row = it.row0 + r, token = row / a.G;
+    finish_row<D, F16, 4>(a, it.first + token, it.kvh * a.G + row - token * a.G, d, x, to, sum);
+  }
+}
+
+template <int D, int R, bool F16>
+cudaError_t launch_join(const PagedArgs& a, int ctas, cudaStream_t s) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas, R, 1);
+  cfg.blockDim = dim3(kJoinThreads, 1, 1);
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, paged_join_kernel<D, R, F16>, a);
 }
 
 }  // namespace
@@ -509,13 +599,26 @@ int attend(const Call& c, const char* what) {
     set_error("%s: the prefix is longer (%lld) than its page table covers", what, (long long)c.prefix_len);
     return QI4_ERR_SHAPE;
   }
-  int sms = 0;
-  rc = require_device(&sms);
-  if (rc) return rc;
   const int D = kv.head_dim;
   const int64_t G = c.Hq / kv.kv_heads;
   // Tokens of a sequence at most, as far as the host knows.
   const int64_t most = c.cu ? (c.max_tokens ? std::min(c.max_tokens, c.T) : c.T) : c.T / c.B;
+  // Units are counted in 32 bits (paged_attention.cuh): tiles of the batch times units of the longest item.
+  {
+    auto units = [&](int64_t tokens, int64_t seqs, int64_t per_seq, int64_t keys) {
+      const int64_t rows = takes_tc(per_seq, G) ? kTcRows / 2 : 8;
+      return (double)(tokens * G / rows + seqs) * kv.kv_heads * (keys / kBlockKeys + 2);
+    };
+    if (units(c.T, c.B, most, (int64_t)kv.table_width * kv.page_size) >= 2147483647.0 ||
+        (prefix && units(c.T, 1, c.T, c.prefix_len) >= 2147483647.0)) {
+      set_error("%s: %lld tokens of %lld sequences over up to %lld keys are too many for one call", what,
+                (long long)c.T, (long long)c.B, (long long)kv.table_width * kv.page_size);
+      return QI4_ERR_SHAPE;
+    }
+  }
+  int sms = 0;
+  rc = require_device(&sms);
+  if (rc) return rc;
   const size_t need = workspace_bytes_for(c.T, c.Hq, kv.kv_heads, D, most, prefix, sms);
   char* ws = static_cast<char*>(c.ws);
   if (ws && (c.ws_bytes < need || !al(ws, 16))) {

@@ -52,9 +52,21 @@ struct SplitItem {
   int pieces, slot, rows, first, row0, kvh;
 };
 
-// CTA c of C owns units [run_start(c), run_start(c + 1)); run_of inverts it.
-__device__ __forceinline__ long long run_start(int c, long long U, int C) { return (long long)c * U / C; }
-__device__ __forceinline__ int run_of(long long u, long long U, int C) { return (int)(((u + 1) * C + U - 1) / U) - 1; }
+// The dealing of U units to C CTAs: CTA c owns [start(c), start(c + 1)),
+// start(c) = floor(c U / C). U below 2^31 (checked on the host), so that
+// nothing needs a 64-bit division.
+struct Runs {
+  int U, C, quot, rest;
+  __device__ __forceinline__ Runs() {}
+  __device__ __forceinline__ Runs(int units, int ctas) : U(units), C(ctas), quot(units / ctas), rest(units - quot * ctas) {}
+  __device__ __forceinline__ int start(int c) const { return c * quot + (int)((unsigned)(c * rest) / (unsigned)C); }
+  __device__ __forceinline__ int holder(int u) const {  // the CTA that owns unit u
+    int c = min(C - 1, (int)((float)u * ((float)C / (float)U)));
+    while (start(c) > u) --c;
+    while (c + 1 < C && start(c + 1) <= u) ++c;
+    return c;
+  }
+};
 
 // One CTA's walk over its units, item by item; every warp keeps its own copy
 // (all lanes alike). A tile has R rows, or the most whole tokens that R rows
@@ -64,8 +76,10 @@ __device__ __forceinline__ int run_of(long long u, long long U, int C) { return 
 // with the next CTA.
 template <int R>
 struct Walk {
-  long long U, u, end, item0;  // u: next unit; item0: the current item's first (fixed-cost) unit
-  int C, tile_rows;
+  Runs runs;
+  int u, end, item0;  // u: next unit; item0: the current item's first (fixed-cost) unit
+  int tile_rows, tile_tokens;
+  unsigned g_inv;     // ceil(2^16 / G): r / G = r g_inv >> 16 for r, G up to 256
   int b, first, n, len, tiles;       // sequence b: first token, tokens, keys, row tiles
   int tile, kvh, blocks, at;         // item; at: next of its 1 + blocks units
   int blk, nblk;                     // this piece: blocks [blk, blk + nblk) of the item
@@ -79,23 +93,26 @@ struct Walk {
     len = min(max(len, 0), a.cap);
     tiles = (n * a.G + tile_rows - 1) / tile_rows;
   }
-  // Keys that a row of the sequence sees.
-  __device__ __forceinline__ int visible(const PagedArgs& a, int seq_row) const {
-    return a.causal ? max(0, min(len, len - n + seq_row / a.G + 1)) : len;
+  // Keys that tile t's last row sees: none beyond is loaded.
+  __device__ __forceinline__ int tile_visible(const PagedArgs& a, int t) const {
+    if (!a.causal) return len;
+    const int last = a.G <= R ? min(n, (t + 1) * tile_tokens) - 1 : (min(n * a.G, (t + 1) * tile_rows) - 1) / a.G;
+    return max(0, min(len, len - n + last + 1));
   }
+  __device__ __forceinline__ int tile_visible(const PagedArgs& a) const { return tile_visible(a, tile); }
   __device__ __forceinline__ int blocks_of(const PagedArgs& a, int t) const {
-    return max(1, (visible(a, min(n * a.G, (t + 1) * tile_rows) - 1) + kBlockKeys - 1) / kBlockKeys);
+    return max(1, (tile_visible(a, t) + kBlockKeys - 1) / kBlockKeys);
   }
   // Units of sequences b0 .. b0 + per - 1, one per group of 32 / per lanes (per
   // a power of two), each lane summing every (32 / per)-th tile; the sum of a
   // sequence ends up in the first lane of its group, 0 in the others.
-  __device__ __forceinline__ long long group_units(const PagedArgs& a, int b0, int per, int lane) {
+  __device__ __forceinline__ int group_units(const PagedArgs& a, int b0, int per, int lane) {
     const int lanes = 32 / per, seq = b0 + lane / lanes, sub = lane % lanes;
-    long long sum = 0;
+    int sum = 0;
     if (seq < a.r.B) {
       load(a, seq);
       if (!a.causal) {
-        if (sub == 0) sum = (long long)tiles * (1 + blocks_of(a, 0));
+        if (sub == 0) sum = tiles * (1 + blocks_of(a, 0));
       } else {
         for (int t = sub; t < tiles; t += lanes) sum += 1 + blocks_of(a, t);
       }
@@ -103,37 +120,36 @@ struct Walk {
     for (int o = lanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     return sub == 0 ? sum * a.Hkv : 0;
   }
-  static __device__ __forceinline__ long long scan(long long x, int lane) {
+  static __device__ __forceinline__ int scan(int x, int lane) {
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long v = __shfl_up_sync(0xffffffffu, x, o);
+      const int v = __shfl_up_sync(0xffffffffu, x, o);
       if (lane >= o) x += v;
     }
     return x;
   }
   // False if the CTA has no units.
   __device__ __forceinline__ bool begin(const PagedArgs& a, int lane) {
-    tile_rows = a.G <= R ? R / a.G * a.G : R;
+    tile_tokens = R / a.G;  // 0 where a token has more rows than a tile
+    tile_rows = a.G <= R ? tile_tokens * a.G : R;
     int per = 32;
     while (per > 1 && per / 2 >= a.r.B) per >>= 1;
-    U = 0;
-    long long mine = 0;
+    g_inv = (65535u + a.G) / (unsigned)a.G;
+    int U = 0, mine = 0;
     for (int b0 = 0; b0 < a.r.B; b0 += per) {
-      long long x = mine = group_units(a, b0, per, lane);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-      U += x;
+      mine = group_units(a, b0, per, lane);
+      U += __reduce_add_sync(0xffffffffu, mine);
     }
-    C = (int)min((long long)gridDim.x, U);
+    const int C = min((int)gridDim.x, U);
     if ((int)blockIdx.x >= C) return false;
-    u = run_start(blockIdx.x, U, C);
-    end = run_start(blockIdx.x + 1, U, C);
+    runs = Runs(U, C);
+    u = runs.start(blockIdx.x);
+    end = runs.start(blockIdx.x + 1);
     // The sequence that holds unit u, then the tile.
-    long long before = 0;
-    int seq = 0;
+    int before = 0, seq = 0;
     for (int b0 = 0; b0 < a.r.B; b0 += per) {
       if (a.r.B > per) mine = group_units(a, b0, per, lane);
-      const long long incl = scan(mine, lane);
+      const int incl = scan(mine, lane);
       const unsigned hit = __ballot_sync(0xffffffffu, before + incl > u);
       if (hit) {
         const int src = __ffs(hit) - 1;
@@ -145,8 +161,8 @@ struct Walk {
     }
     load(a, seq);
     for (tile = 0; tile + 1 < tiles; tile += 32) {
-      const long long units = tile + lane < tiles ? (long long)(1 + blocks_of(a, tile + lane)) * a.Hkv : 0;
-      const long long incl = scan(units, lane);
+      const int units = tile + lane < tiles ? (1 + blocks_of(a, tile + lane)) * a.Hkv : 0;
+      const int incl = scan(units, lane);
       const unsigned hit = __ballot_sync(0xffffffffu, before + incl > u);
       if (hit) {
         const int src = __ffs(hit) - 1;
@@ -157,7 +173,7 @@ struct Walk {
       before += __shfl_sync(0xffffffffu, incl, 31);
     }
     blocks = blocks_of(a, tile);
-    at = (int)(u - before);
+    at = u - before;
     kvh = at / (1 + blocks);
     at -= kvh * (1 + blocks);
     return true;
@@ -180,7 +196,7 @@ struct Walk {
           blocks = blocks_of(a, tile);
         }
       }
-      const int take = (int)min((long long)(1 + blocks - at), end - u);
+      const int take = min(1 + blocks - at, end - u);
       item0 = u - at;
       blk = max(at - 1, 0);
       nblk = at + take - 1 - blk;
@@ -192,17 +208,27 @@ struct Walk {
   __device__ __forceinline__ bool whole() const { return nblk == blocks; }
   __device__ __forceinline__ int rows(const PagedArgs& a) const { return min(tile_rows, n * a.G - tile * tile_rows); }
   __device__ __forceinline__ int row0() const { return tile * tile_rows; }
-  __device__ __forceinline__ int64_t token(const PagedArgs& a, int r) const { return first + (row0() + r) / a.G; }
-  __device__ __forceinline__ int head(const PagedArgs& a, int r) const { return kvh * a.G + (row0() + r) % a.G; }
-  __device__ __forceinline__ int row_visible(const PagedArgs& a, int r) const { return visible(a, row0() + r); }
-  // Keys the tile's last row sees: none beyond is loaded.
-  __device__ __forceinline__ int tile_visible(const PagedArgs& a) const { return row_visible(a, rows(a) - 1); }
+  // Token and query head of row r of the tile.
+  __device__ __forceinline__ void place(const PagedArgs& a, int r, int& token, int& head) const {
+    if (a.G <= R) {
+      const int t = (int)(r * g_inv >> 16);
+      token = first + tile * tile_tokens + t;
+      head = kvh * a.G + r - t * a.G;
+    } else {
+      const int t = (row0() + r) / a.G;
+      token = first + t;
+      head = kvh * a.G + row0() + r - t * a.G;
+    }
+  }
+  __device__ __forceinline__ int row_visible(const PagedArgs& a, int r) const {
+    const int t = a.G <= R ? tile * tile_tokens + (int)(r * g_inv >> 16) : (row0() + r) / a.G;
+    return a.causal ? max(0, min(len, len - n + t + 1)) : len;
+  }
   // Blocks of this piece that hold visible keys: all, but for an item of one empty block.
   __device__ __forceinline__ int loaded(int vis) const { return vis > 0 ? nblk : 0; }
   // The CTAs that hold the item's blocks, and where CTA p's piece lies: its first or its second slot.
-  __device__ __forceinline__ int first_cta() const { return run_of(item0 + 1, U, C); }
-  __device__ __forceinline__ int pieces() const { return run_of(item0 + blocks, U, C) - first_cta() + 1; }
-  __device__ __forceinline__ int slot(int p) const { return 2 * p + (run_start(p, U, C) >= item0 ? 0 : 1); }
+  __device__ __forceinline__ int pieces() const { return runs.holder(item0 + blocks) - runs.holder(item0 + 1) + 1; }
+  __device__ __forceinline__ int slot(int p) const { return 2 * p + (runs.start(p) >= item0 ? 0 : 1); }
 };
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -270,76 +296,6 @@ __device__ __forceinline__ void note_split(const PagedArgs& a, const Walk<R>& w,
   if (any && w.blk == 0 && w.nblk > 0 && !w.whole())
     it = {w.pieces(), w.slot(blockIdx.x), w.rows(a), w.first, w.row0(), w.kvh};
   a.splits[blockIdx.x] = it;
-}
-
-// Joins the pieces of the item that begins in CTA blockIdx.x's run and ends
-// beyond it, if there is one: a group of D / 4 lanes per row, the rows spread
-// over the warps of the blocks (blockIdx.x, 0 ..).
-constexpr int kJoinThreads = 256;
-template <int D, int R, bool F16>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArgs a) {
-  pdl_wait();
-  pdl_launch_dependents();
-  const SplitItem it = a.splits[blockIdx.x];
-  constexpr int kLanes = D / 4, kPerWarp = 32 / kLanes;
-  constexpr int64_t kSlot = (int64_t)R * (D + 2);
-  const int lane = threadIdx.x & 31, d = (lane % kLanes) * 4, np = it.pieces;
-  const float* first = a.ws + it.slot * kSlot;
-  const float* later = a.ws + 2 * (int64_t)blockIdx.x * kSlot;
-  for (int r0 = (blockIdx.y * (kJoinThreads / 32) + threadIdx.x / 32) * kPerWarp; r0 < it.rows;
-       r0 += gridDim.y * (kJoinThreads / 32) * kPerWarp) {
-    const int r = min(r0 + lane / kLanes, it.rows - 1);
-    const int64_t at_ml = (int64_t)R * D + 2 * r, at_acc = (int64_t)r * D + d;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    float top = -INFINITY, l = 0.f;
-    // 32 (16) pieces at a time, one lane each for their maxima and sums; the
-    // running maximum is moved once per round.
-    for (int q0 = 0; q0 < np; q0 += kLanes) {
-      const int p = q0 + lane % kLanes;
-      float2 ml = make_float2(-INFINITY, 0.f);
-      if (p < np) ml = *reinterpret_cast<const float2*>((p ? later + 2 * p * kSlot : first) + at_ml);
-      float m = fmaxf(top, ml.x);
-#pragma unroll
-      for (int o = kLanes / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      const float back = top == -INFINITY ? 0.f : exp2_approx(top - m);
-      top = m;
-      l *= back;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i] *= back;
-      const float fp = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - m);
-      const float lp = ml.y * fp;
-      const int cnt = min(kLanes, np - q0);
-      const float* src = later + 2 * q0 * kSlot + at_acc;
-#pragma unroll 16
-      for (int j = 0; j < cnt; ++j) {
-        const float f = __shfl_sync(0xffffffffu, fp, j, kLanes);
-        l += __shfl_sync(0xffffffffu, lp, j, kLanes);
-        const float4 v = *reinterpret_cast<const float4*>(q0 + j ? src + 2 * j * kSlot : first + at_acc);
-        acc[0] += v.x * f;
-        acc[1] += v.y * f;
-        acc[2] += v.z * f;
-        acc[3] += v.w * f;
-      }
-    }
-    if (r0 + lane / kLanes < it.rows)
-      finish_row<D, F16, 4>(a, it.first + (it.row0 + r) / a.G, it.kvh * a.G + (it.row0 + r) % a.G, d, acc, top, l);
-  }
-}
-
-// Launches the joining of `ctas` runs, behind the kernel that wrote their pieces.
-template <int D, int R, bool F16>
-cudaError_t launch_join(const PagedArgs& a, int ctas, cudaStream_t s) {
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  constexpr int kRowsAtOnce = kJoinThreads / 32 * (128 / D);
-  cfg.gridDim = dim3((unsigned)ctas, (unsigned)((R + 2 * kRowsAtOnce - 1) / (2 * kRowsAtOnce)), 1);
-  cfg.blockDim = dim3(kJoinThreads, 1, 1);
-  cfg.stream = s;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_join_kernel<D, R, F16>, a);
 }
 
 // Launch of the tcgen05 kernel (paged_prefill.cu): tiles of kTcRows rows.

@@ -27,7 +27,6 @@
 //   9         fetches keys and values page by page (TMA, 128-byte swizzle) into
 //             a ring of 128-key slots, keys and values by turns.
 // Tensor memory: scores 2 x 128 columns, sums 2 x D. All waits are bounded.
-#include <algorithm>
 #include <atomic>
 
 #include "paged_attention.cuh"
@@ -302,18 +301,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr int kStep = 128 / (D / 8);  // rows between a thread's chunks
       const int ch = threadIdx.x % (D / 8), r1 = (threadIdx.x % 128) / (D / 8);
       const uint32_t dst = smem_addr(q_s + t * kTileBytes) + (ch >> 3) * kHalf;
+      constexpr int kLoads = D / 8;  // all of a thread's chunks at once
 #pragma unroll
-      for (int g = 0; g < 128 / kStep; g += 8) {
-        uint4 v[8];
+      for (int g = 0; g < 128 / kStep; g += kLoads) {
+        uint4 v[kLoads];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < kLoads; ++i) {
           const int x = t * 128 + r1 + (g + i) * kStep;
           v[i] = make_uint4(0u, 0u, 0u, 0u);
-          if (x < rows)
-            v[i] = *reinterpret_cast<const uint4*>(a.q + w.token(a, x) * a.q_tok + w.head(a, x) * a.q_head + ch * 8);
+          if (x < rows) {
+            int token, head;
+            w.place(a, x, token, head);
+            v[i] = *reinterpret_cast<const uint4*>(a.q + token * a.q_tok + head * a.q_head + ch * 8);
+          }
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < kLoads; ++i) {
           const int qr = r1 + (g + i) * kStep;
           sts128(dst + qr * 128 + (((ch & 7) ^ (qr & 7)) << 4),
                  make_uint4(v[i].x ^ sign, v[i].y ^ sign, v[i].z ^ sign, v[i].w ^ sign));
@@ -336,7 +339,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const bool whole = w.whole(), live = row < rows;
       float* slot = whole ? nullptr : a.ws + (int64_t)w.slot(blockIdx.x) * (kTcRows * (D + 2));
-      const int token = live ? (int)w.token(a, row) : 0, head = live ? w.head(a, row) : 0;
+      int token = 0, head = 0;
+      if (live) w.place(a, row, token, head);
       const int lim = live ? w.row_visible(a, row) : 0, blk0 = w.blk;
       float m = -INFINITY, l = 0.f;
       for (int h = 0; h < 2 * nload; ++h) {  // halves of 64 keys
@@ -440,9 +444,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (whole) {
             finish_row<D, F16, 16>(a, token, head, 16 * c, o, m, l);
           } else {
-            float4* to = reinterpret_cast<float4*>(slot + row * D + 16 * c);
+            // (dims major: a warp's 32 rows side by side)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) to[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+            for (int k = 0; k < 16; ++k) slot[(16 * c + k) * kTcRows + row] = o[k];
           }
         }
       }
@@ -460,8 +464,79 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// Joins the pieces of the item that begins in CTA blockIdx.x's run and ends
+// beyond it, if there is one: block (c, y, z) takes 32 rows and 32 dims. A
+// piece is [D][kTcRows] sums, then [kTcRows] (max, sum): lanes are rows.
+constexpr int kJoinThreads = 256, kMaxPieces = 160;  // at most one piece per CTA
 template <int D, bool F16>
-cudaError_t launch(const CUtensorMap& k, const CUtensorMap& v, const PagedArgs& a, int ctas, cudaStream_t s) {
+__global__ void __launch_bounds__(kJoinThreads) paged_tc_join_kernel(const PagedArgs a) {
+  constexpr int64_t kSlot = (int64_t)kTcRows * (D + 2);
+  __shared__ float f_s[kMaxPieces][32];  // max, then weight of piece p for a row
+  __shared__ float l_s[kMaxPieces][32];
+  __shared__ float out_s[32][33];
+  pdl_wait();
+  pdl_launch_dependents();
+  const SplitItem it = a.splits[blockIdx.x];
+  const int r0 = 32 * blockIdx.y, np = it.pieces;
+  if (r0 >= it.rows) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = r0 + lane;
+  const float* first = a.ws + it.slot * kSlot;
+  const float* later = a.ws + 2 * (int64_t)blockIdx.x * kSlot;
+  for (int p = warp; p < np; p += 8) {
+    const float2 ml =
+        *reinterpret_cast<const float2*>((p ? later + 2 * p * kSlot : first) + (int64_t)kTcRows * D + 2 * r);
+    f_s[p][lane] = ml.x;
+    l_s[p][lane] = ml.y;
+  }
+  __syncthreads();
+  float top = -INFINITY;
+  for (int p = 0; p < np; ++p) top = fmaxf(top, f_s[p][lane]);
+  __syncthreads();
+  const float base = top == -INFINITY ? 0.f : top;
+  for (int p = warp; p < np; p += 8) f_s[p][lane] = exp2_approx(f_s[p][lane] - base);
+  __syncthreads();
+  const int d0 = 4 * warp, d = 32 * blockIdx.z + d0;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
+  for (int p0 = 0; p0 < np; p0 += 4) {
+    float v[4][4], f[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int p = p0 + i;
+      f[i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[i][k] = 0.f;
+      if (p < np) {
+        const float* src = (p ? later + 2 * p * kSlot : first) + (int64_t)d * kTcRows + r;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[i][k] = src[k * kTcRows];
+        f[i] = f_s[p][lane];
+        l += l_s[p][lane] * f[i];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[k] += v[i][k] * f[i];
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) out_s[lane][d0 + k] = acc[k];
+  __syncthreads();  // (every warp is through with the weights, too)
+  if (warp == 0) f_s[0][lane] = top, l_s[0][lane] = l;
+  __syncthreads();
+  const int orow = threadIdx.x / 8, od = (threadIdx.x % 8) * 4;
+  if (r0 + orow < it.rows) {
+    float x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = out_s[orow][od + k];
+    const int row = it.row0 + r0 + orow, token = row / a.G;
+    finish_row<D, F16, 4>(a, it.first + token, it.kvh * a.G + row - token * a.G, 32 * blockIdx.z + od, x,
+                          f_s[0][orow], l_s[0][orow]);
+  }
+}
+
+template <int D, bool F16>
+cudaError_t launch(const CUtensorMap& k, const CUtensorMap& v, const PagedArgs& a, int sms, cudaStream_t s) {
+  const int ctas = sms < kMaxPieces ? sms : kMaxPieces;
   auto kernel = paged_tc_kernel<D, F16>;
   static std::atomic<unsigned long long> configured{0};
   int dev = 0;
@@ -483,7 +558,11 @@ cudaError_t launch(const CUtensorMap& k, const CUtensorMap& v, const PagedArgs& 
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, k, v, a);
-  return e != cudaSuccess ? e : launch_join<D, kTcRows, F16>(a, ctas, s);
+  if (e != cudaSuccess) return e;
+  cfg.gridDim = dim3((unsigned)ctas, kTcRows / 32, D / 32);
+  cfg.blockDim = dim3(kJoinThreads, 1, 1);
+  cfg.dynamicSmemBytes = 0;
+  return cudaLaunchKernelEx(&cfg, paged_tc_join_kernel<D, F16>, a);
 }
 
 }  // namespace
