@@ -523,14 +523,16 @@ cudaError_t launch_kernel(int D, bool f16, int nt, const CUtensorMap& k, const C
   return f16 ? launch_rows<64, true>(nt, k, v, a, ctas, s) : launch_rows<64, false>(nt, k, v, a, ctas, s);
 }
 
-// Rows of one sequence and KV head from which the tcgen05 kernel takes a batch.
+// Rows of one sequence and KV head from which the tcgen05 kernel takes a batch
+// (its tiles hold whole tokens, and its row maxima want a scale that is not
+// negative).
 constexpr int64_t kTcFrom = 65;
-bool takes_tc(int64_t tokens, int64_t G) { return tokens * G >= kTcFrom && G <= 128; }
+bool takes_tc(int64_t tokens, int64_t G, float scale) { return tokens * G >= kTcFrom && G <= 128 && scale >= 0.f; }
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 // Room for the pieces of a launch over `tokens` per sequence, and what the runs note of their split items.
 size_t pieces_bytes(int64_t tokens, int64_t G, int D, int ctas) {
-  const size_t rows = takes_tc(tokens, G) ? kTcRows : 32;
+  const size_t rows = takes_tc(tokens, G, 1.f) ? kTcRows : 32;
   return round256((size_t)ctas * (2 * rows * (D + 2) * sizeof(float) + sizeof(SplitItem)));
 }
 size_t state_bytes(int64_t T, int64_t Hq, int D) { return (size_t)(T * Hq) * (D + 2) * sizeof(float); }
@@ -606,7 +608,7 @@ int attend(const Call& c, const char* what) {
   // Units are counted in 32 bits (paged_attention.cuh): tiles of the batch times units of the longest item.
   {
     auto units = [&](int64_t tokens, int64_t seqs, int64_t per_seq, int64_t keys) {
-      const int64_t rows = takes_tc(per_seq, G) ? kTcRows / 2 : 8;
+      const int64_t rows = takes_tc(per_seq, G, c.scale) ? kTcRows / 2 : 8;
       return (double)(tokens * G / rows + seqs) * kv.kv_heads * (keys / kBlockKeys + 2);
     };
     if (units(c.T, c.B, most, (int64_t)kv.table_width * kv.page_size) >= 2147483647.0 ||
@@ -625,9 +627,13 @@ int attend(const Call& c, const char* what) {
     set_error("%s: the workspace needs %zu bytes, 16-byte aligned (got %zu)", what, need, c.ws_bytes);
     return QI4_ERR_ARGUMENT;
   }
-  CUtensorMap kmap, vmap;
+  CUtensorMap qmap, kmap, vmap;
   const uint32_t box_rows = (uint32_t)std::min(kv.page_size, kBlockKeys);
   if (!tensor_map_pages(&kmap, kv.k, kv, box_rows) || !tensor_map_pages(&vmap, kv.v, kv, box_rows)) return QI4_ERR_LAUNCH;
+  if (takes_tc(prefix ? c.T : most, G, c.scale) &&
+      !tensor_map_rows3(&qmap, c.q, kv.dtype == QI4_DTYPE_F16, D, c.Hq, c.T, c.q_head, c.q_tok, (uint32_t)G,
+                        (uint32_t)(kTcRows / G)))
+    return QI4_ERR_LAUNCH;
   void* own = nullptr;
   if (!ws) {
     if (scratch_alloc(&own, need, c.stream) != cudaSuccess) {
@@ -650,11 +656,11 @@ int attend(const Call& c, const char* what) {
   // One launch: pieces at `at`, the kernel for `tokens` per sequence. The
   // mma.sync tile is the smallest of 8, 16 and 32 rows that holds them.
   auto launch = [&](PagedArgs& x, char* at, int64_t tokens) {
-    const bool tc = takes_tc(tokens, G);
-    const size_t rows = tc ? kTcRows : 32;
+    const bool tc = takes_tc(tokens, G, c.scale);
+    const size_t rows = takes_tc(tokens, G, 1.f) ? kTcRows : 32;
     x.ws = reinterpret_cast<float*>(at);
     x.splits = reinterpret_cast<SplitItem*>(at + (size_t)sms * 2 * rows * (D + 2) * sizeof(float));
-    if (tc) return launch_paged_tc(D, f16, kmap, vmap, x, sms, c.stream);
+    if (tc) return launch_paged_tc(D, f16, qmap, kmap, vmap, x, sms, c.stream);
     return launch_kernel(D, f16, tokens * G <= 8 ? 1 : tokens * G <= 16 ? 2 : 4, kmap, vmap, x, sms, c.stream);
   };
   float* state = nullptr;

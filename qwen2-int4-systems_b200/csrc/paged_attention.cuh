@@ -300,8 +300,9 @@ __device__ __forceinline__ void note_split(const PagedArgs& a, const Walk<R>& w,
 
 // Launch of the tcgen05 kernel (paged_prefill.cu): tiles of kTcRows rows.
 constexpr int kTcRows = 256;
-cudaError_t launch_paged_tc(int D, bool f16, const CUtensorMap& k, const CUtensorMap& v, const PagedArgs& a, int ctas,
-                            cudaStream_t s);
+// q: the queries as (dims, heads, tokens), box {64, G, kTcRows / G}.
+cudaError_t launch_paged_tc(int D, bool f16, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
+                            const PagedArgs& a, int ctas, cudaStream_t s);
 
 // One box {64 dims, rows, one head, one page} of the pool into shared memory.
 __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int slot, int head, int page,

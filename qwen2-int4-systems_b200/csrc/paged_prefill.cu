@@ -17,15 +17,20 @@
 //             sum of the weights stays FP32 and unrounded). The weights are
 //             taken relative to a row maximum that is moved only when a score
 //             exceeds it by more than 2^8 (exponents leave room): the sums in
-//             tensor memory are then rescaled, rarely. Also the queries (plain
-//             loads, swizzled stores) and the epilogue.
+//             tensor memory are then rescaled, rarely. Also the epilogue.
 //   8         issues the products: S = Q K^T (both operands from shared
 //             memory), O += P V (P from tensor memory, V as it lies in the
 //             page: key-major, the descriptor's transposed form). Products
 //             execute in the order of issue, so "scores of unit i are there"
 //             also says that the sums of unit i - 1 are.
-//   9         fetches keys and values page by page (TMA, 128-byte swizzle) into
-//             a ring of 128-key slots, keys and values by turns.
+//   9         fetches the queries (one TMA box of whole tokens per 64 dims) and,
+//             page by page, keys and values into a ring of 128-key slots, keys
+//             and values by turns (128-byte swizzle throughout).
+// The weights of a unit are announced in two halves of 64 keys, so that the
+// first half's product runs under the second half's exponentials. (Scores in
+// halves of 64 columns as well, to have one half's always ready, took longer:
+// a product of N = 64 with both operands in shared memory takes the 64 cycles
+// of one with N = 128.)
 // Tensor memory: scores 2 x 128 columns, sums 2 x D. All waits are bounded.
 #include <atomic>
 
@@ -44,7 +49,7 @@ constexpr int slot_bytes(int D) { return kBlockKeys * D * 2; }
 constexpr int ring_slots(int D) { return D == 128 ? 5 : 10; }
 constexpr size_t smem_of(int D) {
   return 1024 + (size_t)kTcRows * D * 2 + (size_t)ring_slots(D) * slot_bytes(D) +
-         (16 + 2 * ring_slots(D)) * sizeof(uint64_t) + 16;
+         (12 + 2 * ring_slots(D)) * sizeof(uint64_t) + 16;
 }
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -138,17 +143,18 @@ __host__ __device__ constexpr uint32_t idesc(bool f16, int N, bool v) {
 
 template <int D, bool F16>
 __global__ void __launch_bounds__(kThreads, 1)
-    paged_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
-                    const PagedArgs a) {
+    paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                    const __grid_constant__ CUtensorMap vmap, const PagedArgs a) {
   constexpr int kSlots = ring_slots(D), kSlotBytes = slot_bytes(D), kHalf = kBlockKeys * 128;
-  constexpr int kTileBytes = 128 * D * 2;
+  constexpr int kTileBytes = 128 * 128, kQHalf = kTcRows * 128;  // 128 rows, and 256 rows, of 64 dims
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
-  uint8_t* q_s = smem;                      // 2 tiles [D / 64][128 rows][128 B]
-  uint8_t* ring = smem + 2 * kTileBytes;    // slots [D / 64][128 keys][128 B]
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(ring + kSlots * kSlotBytes);  // [2] 4 warps
-  uint64_t* s_full = q_full + 2;                                               // [2 tiles][2 halves] commit
-  uint64_t* p_full = s_full + 4;                                               // [2][2] 4 warps
+  uint8_t* q_s = smem;                      // [D / 64][256 rows][128 B]: the tiles are its row halves
+  uint8_t* ring = smem + kTcRows * D * 2;   // slots [D / 64][128 keys][128 B]
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(ring + kSlots * kSlotBytes);  // TMA
+  uint64_t* q_empty = q_full + 1;                                              // commit
+  uint64_t* s_full = q_empty + 1;                                              // [2 tiles] commit
+  uint64_t* p_full = s_full + 2;                                               // [2][2 halves] 4 warps
   uint64_t* o_done = p_full + 4;                                               // [2] commit, per half
   uint64_t* o_full = o_done + 2;                                               // [2] commit, per item
   uint64_t* kv_full = o_full + 2;                                              // [kSlots] TMA
@@ -158,19 +164,19 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], 4);
+      mbar_init(&s_full[i], 1);
       mbar_init(&o_done[i], 1);
       mbar_init(&o_full[i], 1);
     }
-    for (int i = 0; i < 4; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
-    }
+    for (int i = 0; i < 4; ++i) mbar_init(&p_full[i], 4);
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
     for (int i = 0; i < kSlots; ++i) {
       mbar_init(&kv_full[i], 1);
       mbar_init(&kv_empty[i], 1);
     }
     fence_barrier_init();
+    prefetch_tensor_map(&qmap);
     prefetch_tensor_map(&kmap);
     prefetch_tensor_map(&vmap);
   }
@@ -188,8 +194,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---- producer ----
     const int box_rows = 1 << a.box_shift;
     int pos = 0;  // ring position
+    uint32_t nq = 0;
     while (w.next(a)) {
       const int vis = w.tile_visible(a);
+      if (w.loaded(vis) > 0) {
+        // The tile's queries: whole tokens of the KV head's G query heads are its rows in order. Tokens of the next
+        // sequence that come with a sequence's last tile, and rows past the box, only make rows that nobody reads.
+        mbar_wait(q_empty, (nq++ & 1u) ^ 1u, &g_paged_tc_error);
+        if (lane == 0) {
+          mbar_arrive_expect_tx(q_full, (uint32_t)(w.tile_rows * D * 2));
+#pragma unroll
+          for (int h = 0; h < D / 64; ++h)
+            tma_load_3d(q_s + h * kQHalf, &qmap, 64 * h, w.kvh * a.G, w.first + w.tile * w.tile_tokens, q_full);
+        }
+        __syncwarp();
+      }
       if (lane == 0 && a.fixed_len < 0 && __ldg(a.r.lengths + w.b) > a.cap)
         atomicOr(&g_paged_tc_error, kErrCacheFull);
       int win0 = -1, win = -1;
@@ -222,23 +241,23 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (any && warp == kSoftmaxWarps) {
     // ---- products ----
     // The whole warp runs the loops and the waits; one lane issues.
-    constexpr uint32_t s_id = idesc(F16, 64, false), o_id = idesc(F16, D, true);
+    constexpr uint32_t s_id = idesc(F16, kBlockKeys, false), o_id = idesc(F16, D, true);
     const uint64_t q_desc = sw128_desc(smem_addr(q_s)), k_desc = sw128_desc(smem_addr(ring)),
                    v_desc0 = v_desc<D>(smem_addr(ring));  // (descriptors count addresses in 16 bytes)
     int pos = 0;
-    uint32_t nq[2] = {0, 0}, np[2] = {0, 0};  // uses of q_full, and of p_full of either half
-    // Scores of tile t and the keys of half x of slot st; frees the slot behind the last.
-    auto scores = [&](int t, int x, int st, bool last) {
+    uint32_t nq = 0, np[2] = {0, 0};  // uses of q_full, and of p_full of either half
+    // Scores of tile t and the keys of slot st; `last`: frees the slot, and `done` the queries.
+    auto scores = [&](int t, int st, bool last, bool done) {
       tc_fence_after();
       if (elect_one()) {
-        const uint64_t qd = q_desc + t * (kTileBytes >> 4), kd = k_desc + (st * kSlotBytes + x * 64 * 128) / 16;
+        const uint64_t qd = q_desc + t * (kTileBytes >> 4), kd = k_desc + st * (kSlotBytes >> 4);
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t at = ((k / 4) * kHalf + (k % 4) * 32) >> 4;
-          tc_mma(tmem + 128 * t + 64 * x, qd + at, kd + at, s_id, k > 0);
-        }
-        tc_commit(&s_full[2 * t + x]);
+        for (int k = 0; k < D / 16; ++k)
+          tc_mma(tmem + 128 * t, qd + (((k / 4) * kQHalf + (k % 4) * 32) >> 4),
+                 kd + (((k / 4) * kHalf + (k % 4) * 32) >> 4), s_id, k > 0);
+        tc_commit(&s_full[t]);
         if (last) tc_commit(&kv_empty[st]);
+        if (done) tc_commit(q_empty);
       }
       __syncwarp();
     };
@@ -248,23 +267,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int nt = w.rows(a) > 128 ? 2 : 1;
       const int k0 = pos % kSlots;
       mbar_wait(&kv_full[k0], (uint32_t)(pos / kSlots) & 1u, &g_paged_tc_error);
-      for (int t = 0; t < nt; ++t) {
-        mbar_wait(&q_full[t], nq[t]++ & 1u, &g_paged_tc_error);
-        scores(t, 0, k0, false);
-      }
-      for (int t = 0; t < nt; ++t) scores(t, 1, k0, t == nt - 1);
+      mbar_wait(q_full, nq++ & 1u, &g_paged_tc_error);
+      for (int t = 0; t < nt; ++t) scores(t, k0, t == nt - 1, t == nt - 1 && nload == 1);
       ++pos;
       for (int i = 0; i < nload; ++i) {
         const bool more = i + 1 < nload;
         const int vs = pos % kSlots, ks = (pos + 1) % kSlots;
+        const uint64_t vd = v_desc0 + vs * (kSlotBytes >> 4);
+        for (int t = 0; t < nt; ++t) {
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
-          for (int t = 0; t < nt; ++t) {
+          for (int x = 0; x < 2; ++x) {
             mbar_wait(&p_full[2 * t + x], np[t] & 1u, &g_paged_tc_error);
             if (x == 0 && t == 0) mbar_wait(&kv_full[vs], (uint32_t)(pos / kSlots) & 1u, &g_paged_tc_error);
             tc_fence_after();
             if (elect_one()) {
-              const uint64_t vd = v_desc0 + vs * (kSlotBytes >> 4);
 #pragma unroll
               for (int k = 0; k < 4; ++k)
                 tc_mma_ta(tmem + 256 + D * t, tmem + 128 * t + 64 * x + 8 * k, vd + (4 * x + k) * (2048 >> 4), o_id,
@@ -274,12 +290,13 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (x == 1 && t == nt - 1) tc_commit(&kv_empty[vs]);
             }
             __syncwarp();
-            if (x == 1) ++np[t];
-            if (more) {
-              if (x == 0 && t == 0) mbar_wait(&kv_full[ks], (uint32_t)((pos + 1) / kSlots) & 1u, &g_paged_tc_error);
-              scores(t, x, ks, x == 1 && t == nt - 1);
-            }
           }
+          ++np[t];
+          if (more) {
+            if (t == 0) mbar_wait(&kv_full[ks], (uint32_t)((pos + 1) / kSlots) & 1u, &g_paged_tc_error);
+            scores(t, ks, t == nt - 1, t == nt - 1 && i + 2 == nload);
+          }
+        }
         pos += more ? 2 : 1;
       }
     }
@@ -289,52 +306,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int row = t * 128 + r;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_tm = tmem + 128 * t + lanes, o_tm = tmem + 256 + D * t + lanes;
-    // The row maximum is taken of the raw scores: a negative scale turns the queries' signs.
-    const uint32_t sign = a.scale_log2 < 0.f ? 0x80008000u : 0u;
-    const float scale = fmaxf(fabsf(a.scale_log2), 1e-30f);
+    // The row maximum is taken of the raw scores (the scale is not negative here; never zero, which would make
+    // a hidden key's -inf a NaN).
+    const float scale = fmaxf(a.scale_log2, 1e-30f);
     int pos = 0;
-    uint32_t ns = 0, no = 0, done = 0;  // uses of s_full (of either half), o_full, and o_done
-    // The queries of the walk's item into this tile's shared memory, 16-byte chunks, rows past the last zero.
-    auto queries = [&]() {
-      const int rows = w.rows(a);
-      if (t * 128 >= rows || w.loaded(w.tile_visible(a)) == 0) return;
-      constexpr int kStep = 128 / (D / 8);  // rows between a thread's chunks
-      const int ch = threadIdx.x % (D / 8), r1 = (threadIdx.x % 128) / (D / 8);
-      const uint32_t dst = smem_addr(q_s + t * kTileBytes) + (ch >> 3) * kHalf;
-      constexpr int kLoads = D / 8;  // all of a thread's chunks at once
-#pragma unroll
-      for (int g = 0; g < 128 / kStep; g += kLoads) {
-        uint4 v[kLoads];
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-          const int x = t * 128 + r1 + (g + i) * kStep;
-          v[i] = make_uint4(0u, 0u, 0u, 0u);
-          if (x < rows) {
-            int token, head;
-            w.place(a, x, token, head);
-            v[i] = *reinterpret_cast<const uint4*>(a.q + token * a.q_tok + head * a.q_head + ch * 8);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-          const int qr = r1 + (g + i) * kStep;
-          sts128(dst + qr * 128 + (((ch & 7) ^ (qr & 7)) << 4),
-                 make_uint4(v[i].x ^ sign, v[i].y ^ sign, v[i].z ^ sign, v[i].w ^ sign));
-        }
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&q_full[t]);
-    };
+    uint32_t ns = 0, no = 0, done = 0;  // uses of s_full, o_full, and o_done
     bool have = any && w.next(a);
-    if (have) queries();
     while (have) {
       const int rows = w.rows(a), vis = w.tile_visible(a), nload = w.loaded(vis);
       const int base_pos = pos;
       pos += 2 * nload;
       if (t * 128 >= rows) {
         have = w.next(a);
-        if (have) queries();
         continue;
       }
       const bool whole = w.whole(), live = row < rows;
@@ -346,8 +329,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int h = 0; h < 2 * nload; ++h) {  // halves of 64 keys
         const int x = h & 1, key0 = (blk0 + (h >> 1)) * kBlockKeys + 64 * x;
         const uint32_t s_at = s_tm + 64 * x;
-        mbar_wait(&s_full[2 * t + x], ns & 1u, &g_paged_tc_error);
-        ns += x;
+        if (x == 0) mbar_wait(&s_full[t], ns++ & 1u, &g_paged_tc_error);
         tc_fence_after();
         float s[64];
         tmem_ld(s_at, s);
@@ -369,8 +351,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (__any_sync(0xffffffffu, move)) {
           const float to = move ? top : m;
           if (h > 0) {
-            // The sums of the half before must be complete (phase done + h - 1); those of the halves before it are,
-            // as the scores just read were issued behind them, so the phase's parity says which one it is.
+            // The sums of the half before must be complete (phase done + h - 1). Those of the unit before are, as
+            // this unit's scores were issued behind them, so the parity says which phase it is.
             mbar_wait(&o_done[t], (done + h - 1) & 1u, &g_paged_tc_error);
             tc_fence_after();
             const float f = move ? exp2_approx(m - to) : 1.f;
@@ -421,10 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[2 * t + x]);
       }
-      // All scores of this item have been read, so the next one's queries may replace its own; the products go on
-      // with it while the sums of this one are written out.
       have = w.next(a);
-      if (have) queries();
       if (nload > 0) {
         done += 2 * nload;
         mbar_wait(&o_full[t], no++ & 1u, &g_paged_tc_error);
@@ -535,7 +514,8 @@ __global__ void __launch_bounds__(kJoinThreads) paged_tc_join_kernel(const Paged
 }
 
 template <int D, bool F16>
-cudaError_t launch(const CUtensorMap& k, const CUtensorMap& v, const PagedArgs& a, int sms, cudaStream_t s) {
+cudaError_t launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const PagedArgs& a, int sms,
+                   cudaStream_t s) {
   const int ctas = sms < kMaxPieces ? sms : kMaxPieces;
   auto kernel = paged_tc_kernel<D, F16>;
   static std::atomic<unsigned long long> configured{0};
@@ -557,7 +537,7 @@ cudaError_t launch(const CUtensorMap& k, const CUtensorMap& v, const PagedArgs& 
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, k, v, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, q, k, v, a);
   if (e != cudaSuccess) return e;
   cfg.gridDim = dim3((unsigned)ctas, kTcRows / 32, D / 32);
   cfg.blockDim = dim3(kJoinThreads, 1, 1);
@@ -569,10 +549,10 @@ cudaError_t launch(const CUtensorMap& k, const CUtensorMap& v, const PagedArgs& 
 
 int read_paged_tc_error(cudaStream_t stream) { return read_error_word(&g_paged_tc_error, stream); }
 
-cudaError_t launch_paged_tc(int D, bool f16, const CUtensorMap& k, const CUtensorMap& v, const PagedArgs& a, int ctas,
-                            cudaStream_t s) {
-  if (D == 128) return f16 ? launch<128, true>(k, v, a, ctas, s) : launch<128, false>(k, v, a, ctas, s);
-  return f16 ? launch<64, true>(k, v, a, ctas, s) : launch<64, false>(k, v, a, ctas, s);
+cudaError_t launch_paged_tc(int D, bool f16, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
+                            const PagedArgs& a, int ctas, cudaStream_t s) {
+  if (D == 128) return f16 ? launch<128, true>(q, k, v, a, ctas, s) : launch<128, false>(q, k, v, a, ctas, s);
+  return f16 ? launch<64, true>(q, k, v, a, ctas, s) : launch<64, false>(q, k, v, a, ctas, s);
 }
 
 }  // namespace qi4

@@ -163,4 +163,29 @@ bool tensor_map_pages(CUtensorMap* out, const void* base, const qi4_paged_kv& kv
   return true;
 }
 
+bool tensor_map_rows3(CUtensorMap* out, const void* base, bool f16, int64_t dims, int64_t heads, int64_t rows,
+                      int64_t head_stride, int64_t row_stride, uint32_t box_heads, uint32_t box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) {
+    set_error("cuTensorMapEncodeTiled is not available from the driver");
+    return false;
+  }
+  auto stride = [](int64_t elements, int64_t count) { return (cuuint64_t)(count > 1 ? elements * 2 : 16); };
+  const cuuint64_t d[3] = {(cuuint64_t)dims, (cuuint64_t)heads, (cuuint64_t)rows};
+  const cuuint64_t strides[2] = {stride(head_stride, heads), stride(row_stride, rows)};
+  const cuuint32_t box[3] = {64, box_heads, box_rows}, estr[3] = {1, 1, 1};
+  alignas(64) CUtensorMap map;
+  const CUresult r = fn(&map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                        const_cast<void*>(base), d, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed (%d) for %lld x %lld x %lld rows", (int)r, (long long)rows,
+              (long long)heads, (long long)dims);
+    return false;
+  }
+  *out = map;
+  return true;
+}
+
 }  // namespace qi4

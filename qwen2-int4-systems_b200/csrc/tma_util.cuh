@@ -39,6 +39,12 @@ bool tensor_map_row_boxes(CUtensorMap* out, const void* base, uint64_t row_bytes
 // box_rows slots and 128-byte swizzle. Encoded anew for every call.
 bool tensor_map_pages(CUtensorMap* out, const void* base, const qi4_paged_kv& kv, uint32_t box_rows);
 
+// A [rows][heads][dims] 16-bit array (dims contiguous, strides in elements) as
+// a 3-D map (dims, heads, rows) with a box of 64 dims x box_heads x box_rows
+// and 128-byte swizzle. Encoded anew for every call.
+bool tensor_map_rows3(CUtensorMap* out, const void* base, bool f16, int64_t dims, int64_t heads, int64_t rows,
+                      int64_t head_stride, int64_t row_stride, uint32_t box_heads, uint32_t box_rows);
+
 // Device-side error flags (one per translation unit), read and cleared on host.
 constexpr int kErrWaitTimeout = 1;
 
