@@ -388,18 +388,22 @@ QI4_API int qi4_bf16_argmax_rows(const void* logits, int64_t B, int64_t V, int64
  * A batch of B sequences brings T new tokens, the rows of [T, heads, dim]
  * tensors: sequence b owns rows cu_tokens[b] .. cu_tokens[b + 1] - 1 (device,
  * int32, B + 1 entries, ascending; a sequence may have none), or T / B rows
- * each when cu_tokens is NULL.
+ * each when cu_tokens is NULL. Results in rows that no sequence owns are not
+ * defined.
  *
  * No device array can make a kernel touch memory outside the tensors: token
  * ranges are clipped to T, positions beyond the table and pages outside the
  * pool are not written (and read as zeros), and qi4_device_status reports
  * QI4_DEVICE_CACHE_FULL (position beyond the block table), QI4_DEVICE_BAD_PAGE,
  * QI4_DEVICE_BAD_POSITION (no such row of cos / sin; the nearest is used) and
- * QI4_DEVICE_BAD_TOKEN (a drafted token outside the vocabulary).
+ * QI4_DEVICE_BAD_TOKEN (a drafted token outside the vocabulary) and
+ * QI4_DEVICE_TOO_MANY_TOKENS (a sequence with more new tokens than max_tokens
+ * says; rows of its further tokens may not have been computed).
  */
 #define QI4_DEVICE_BAD_PAGE 4
 #define QI4_DEVICE_BAD_POSITION 8
 #define QI4_DEVICE_BAD_TOKEN 16
+#define QI4_DEVICE_TOO_MANY_TOKENS 32
 typedef struct qi4_paged_kv {
   void* k;
   void* v;
@@ -448,8 +452,8 @@ QI4_API int qi4_rope_paged_append(const qi4_paged_kv* kv, const void* q, int64_t
  * beyond a length hold does not matter, NaN included. q as in
  * qi4_rope_paged_append; out [T, Hq, head_dim] contiguous, 32-byte aligned;
  * head_dim 64 or 128.
- * max_tokens: no sequence has more new tokens (0: not known); it only chooses
- * the kernel. workspace: qi4_paged_attention_workspace bytes, 16-byte aligned,
+ * max_tokens: no sequence has more new tokens (0: not known); it chooses the
+ * kernel and its tiles. workspace: qi4_paged_attention_workspace bytes, 16-byte aligned,
  * no initialisation needed, not shared by calls that may overlap; NULL: the
  * library's scratch pool. Replaces, for a paged cache, reference
  * src/qwen_int4/model.py:90-118.

@@ -11,8 +11,8 @@
 // of them: 192 KB in flight per SM, four times what the HBM latency asks for.
 // Eight warps take 16 keys each on mma.sync, keys as the 16 rows and the query
 // rows as columns of 8, so 6 query heads of a KV head waste 2 columns and not
-// 10. Scores S^T = K Q^T, a softmax with running max per warp on the score
-// registers, O^T += V^T P^T with P split into a 16-bit value and its 16-bit
+// 10. Scores S^T = K Q^T, a softmax on the score registers with a maximum per
+// warp that moves only when a score exceeds it by more than 2^8, O^T += V^T P^T with P split into a 16-bit value and its 16-bit
 // remainder (the products keep 16 bits or more of each weight; the second
 // product is hidden behind the loads). The warps' sums meet in the stage of
 // the item's last unit, which is released afterwards.
@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   // The next launch may be scheduled once every CTA has passed its own wait:
   // what it reads before its wait is then older than this launch.
-  pdl_wait();
+  if (!a.late) pdl_wait();
   pdl_launch_dependents();
 
   Walk<R> w;
@@ -117,6 +117,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int vis = w.tile_visible(a);
       const int nload = w.loaded(vis);
       if (lane == 0 && a.fixed_len < 0 && __ldg(a.r.lengths + w.b) > a.cap) atomicOr(&g_paged_error, kErrCacheFull);
+      if (lane == 0 && a.one_tile && w.n * a.G > a.tile_rows) atomicOr(&g_paged_error, QI4_DEVICE_TOO_MANY_TOKENS);
       int win0 = -1, win = -1;  // table entries win0 .. win0 + 31, one per lane
       for (int i = 0; i < nload; ++i) {
         const int key0 = (w.blk + i) * kBlockKeys;
@@ -149,6 +150,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
+    if (lane == 0) note_split(a, w, true);
     return;
   }
 
@@ -160,6 +162,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   while (w.next(a)) {
     const int rows = w.rows(a), vis = w.tile_visible(a), nload = w.loaded(vis);
     if (nload == 0) {  // no row sees a key
+      if (a.late) pdl_wait();
       for (int i = threadIdx.x; i < rows * (D / 4); i += 32 * kWarps) {
         const int r = i / (D / 4);
         float none[4] = {0.f, 0.f, 0.f, 0.f};
@@ -249,36 +252,51 @@ __global__ void __launch_bounds__(kThreads, 1)
               mma16816<F16>(sc[nt], ka[1], q2, q3);
             }
           }
-          uint32_t ph[NT][2], pl[NT][2];
+          // Hidden keys, and whether a score leaves its row's maximum more than 2^8 behind.
           const bool masked = key0 + 16 > lim_min;
+          bool move = false;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            float alpha[2], p[4];
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              float x0 = sc[nt][e] * a.scale_log2, x1 = sc[nt][2 + e] * a.scale_log2;
+              float &x0 = sc[nt][e], &x1 = sc[nt][2 + e];
+              x0 *= a.scale_log2, x1 *= a.scale_log2;
               if (masked || lim[nt][e] == 0) {
                 x0 = key0 + gq < lim[nt][e] ? x0 : -INFINITY;
                 x1 = key0 + gq + 8 < lim[nt][e] ? x1 : -INFINITY;
               }
-              float t = fmaxf(x0, x1);
-              t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
-              t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
-              t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
-              const float mn = fmaxf(m[nt][e], t);
-              const float base = mn == -INFINITY ? 0.f : mn;
-              alpha[e] = exp2_approx(m[nt][e] - base);
-              m[nt][e] = mn;
-              p[e] = exp2_approx(x0 - base);
-              p[2 + e] = exp2_approx(x1 - base);
-              l[nt][e] = l[nt][e] * alpha[e] + (p[e] + p[2 + e]);  // this lane's keys; summed over gq at the end
+              move |= fmaxf(x0, x1) > m[nt][e] + 8.f;
             }
+          if (__any_sync(0xffffffffu, move)) {
+            // The maxima move (in the first unit, and rarely after it): the sums so far are rescaled.
 #pragma unroll
-            for (int mt = 0; mt < D / 16; ++mt) {
-              o[mt][nt][0] *= alpha[0];
-              o[mt][nt][1] *= alpha[1];
-              o[mt][nt][2] *= alpha[0];
-              o[mt][nt][3] *= alpha[1];
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                float t = fmaxf(sc[nt][e], sc[nt][2 + e]);
+                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
+                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
+                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
+                const float mn = fmaxf(m[nt][e], t), alpha = mn == -INFINITY ? 1.f : exp2_approx(m[nt][e] - mn);
+                m[nt][e] = mn;
+                l[nt][e] *= alpha;
+#pragma unroll
+                for (int mt = 0; mt < D / 16; ++mt) {
+                  o[mt][nt][e] *= alpha;
+                  o[mt][nt][2 + e] *= alpha;
+                }
+              }
+          }
+          uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float p[4];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float base = m[nt][e] == -INFINITY ? 0.f : m[nt][e];
+              p[e] = exp2_approx(sc[nt][e] - base);
+              p[2 + e] = exp2_approx(sc[nt][2 + e] - base);
+              l[nt][e] += p[e] + p[2 + e];  // this lane's keys; summed over gq at the end
             }
             const uint32_t h0 = pack2<F16>(p[0], p[1]), h1 = pack2<F16>(p[2], p[3]);
             const float2 f0 = unpack2<F16>(h0), f1 = unpack2<F16>(h1);
@@ -327,9 +345,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       named_barrier(1, 32 * kWarps);  // every warp is done with the held stage
-      // Four buffers [R][D], dims swizzled so that the fragments' stores spread over the banks.
+      // Buffers [R][D], dims swizzled so that the fragments' stores spread over the banks: one per warp where they
+      // fit the stage, else one for each of four warps, which add theirs to another's.
+      constexpr int kBuffers = NT <= 2 ? kWarps : kWarps / 2;
       float* buf = reinterpret_cast<float*>(smem + held * kStageBytes);
-      static_assert(4 * R * D * sizeof(float) <= (size_t)stage_bytes(D), "the sums must fit one stage");
+      static_assert(kBuffers * R * D * sizeof(float) <= (size_t)stage_bytes(D), "the sums must fit one stage");
       float f[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -340,10 +360,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int x = 0; x < kWarps; ++x) top = fmaxf(top, rm[x * R + nt * 8 + 2 * tq + e]);
           f[nt][e] = m[nt][e] == -INFINITY ? 0.f : exp2_approx(m[nt][e] - top);
         }
-      float* mine = buf + (warp & 3) * R * D;
+      float* mine = buf + (warp % kBuffers) * R * D;
 #pragma unroll
-      for (int round = 0; round < 2; ++round) {
-        if ((warp >= 4) == (round == 0)) {
+      for (int round = 0; round < kWarps / kBuffers; ++round) {
+        if (kBuffers == kWarps || (warp >= kBuffers) == (round == 0)) {
 #pragma unroll
           for (int mt = 0; mt < D / 16; ++mt)
 #pragma unroll
@@ -359,6 +379,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         named_barrier(1, 32 * kWarps);
       }
       constexpr int kLanes = D / 4;
+      if (a.late) pdl_wait();
       const bool whole = w.whole();
       float* slot = whole ? nullptr : a.ws + (int64_t)w.slot(blockIdx.x) * (R * (D + 2));
       for (int i = threadIdx.x; i < rows * kLanes; i += 32 * kWarps) {
@@ -371,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           sum += rm[x * R + r] == -INFINITY ? 0.f : rl[x * R + r] * exp2_approx(rm[x * R + r] - top);
         float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
+        for (int x = 0; x < kBuffers; ++x) {
           const float4 v = *reinterpret_cast<const float4*>(buf + (x * R + r) * D + (d ^ (((r >> 1) & 3) << 3)));
           acc[0] += v.x, acc[1] += v.y, acc[2] += v.z, acc[3] += v.w;
         }
@@ -390,7 +411,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       par ^= 1;
     }
   }
-  if (threadIdx.x == 0) note_split(a, w, true);
 }
 
 // Joins the pieces of the item that begins in CTA blockIdx.x's run and ends
@@ -404,8 +424,8 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArg
   constexpr int64_t kSlot = (int64_t)R * (D + 2);
   __shared__ float4 acc_s[kGroups][kLanes];
   __shared__ float2 ml_s[kGroups];
+  pdl_launch_dependents();  // (what follows waits for this launch, and it for the one before)
   pdl_wait();
-  pdl_launch_dependents();
   const SplitItem it = a.splits[blockIdx.x];
   const int r = blockIdx.y, np = it.pieces;
   if (r >= it.rows) return;
@@ -457,7 +477,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArg
       sum += ml_s[g].y * f;
       x[0] += v.x * f, x[1] += v.y * f, x[2] += v.z * f, x[3] += v.w * f;
     }
-    const int row = it.row0 + r, token = row / a.G;
+    const int row = it.row0 + r, token = a.by_G(row);
     finish_row<D, F16, 4>(a, it.first + token, it.kvh * a.G + row - token * a.G, d, x, to, sum);
   }
 }
@@ -514,6 +534,7 @@ cudaError_t launch_rows(int nt, const CUtensorMap& k, const CUtensorMap& v, cons
                         cudaStream_t s) {
   if (nt == 1) return launch_decode<D, 1, F16>(k, v, a, ctas, s);
   if (nt == 2) return launch_decode<D, 2, F16>(k, v, a, ctas, s);
+  if (nt == 3) return launch_decode<D, 3, F16>(k, v, a, ctas, s);
   return launch_decode<D, 4, F16>(k, v, a, ctas, s);
 }
 
@@ -526,7 +547,7 @@ cudaError_t launch_kernel(int D, bool f16, int nt, const CUtensorMap& k, const C
 // Rows of one sequence and KV head from which the tcgen05 kernel takes a batch
 // (its tiles hold whole tokens, and its row maxima want a scale that is not
 // negative).
-constexpr int64_t kTcFrom = 65;
+constexpr int64_t kTcFrom = 33;
 bool takes_tc(int64_t tokens, int64_t G, float scale) { return tokens * G >= kTcFrom && G <= 128 && scale >= 0.f; }
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
@@ -654,32 +675,41 @@ int attend(const Call& c, const char* what) {
   const bool f16 = kv.dtype == QI4_DTYPE_F16;
   cudaError_t e = cudaSuccess;
   // One launch: pieces at `at`, the kernel for `tokens` per sequence. The
-  // mma.sync tile is the smallest of 8, 16 and 32 rows that holds them.
+  // mma.sync tile is the smallest of 8, 16, 24 and 32 rows that holds them.
   auto launch = [&](PagedArgs& x, char* at, int64_t tokens) {
     const bool tc = takes_tc(tokens, G, c.scale);
     const size_t rows = takes_tc(tokens, G, 1.f) ? kTcRows : 32;
     x.ws = reinterpret_cast<float*>(at);
+    const int R = tc ? kTcRows : tokens * G <= 8 ? 8 : tokens * G <= 16 ? 16 : tokens * G <= 24 ? 24 : 32;
+    x.tile_tokens = (int)(R / G);
+    x.tile_rows = G <= R ? x.tile_tokens * (int)G : R;
+    x.one_tile = tokens * G <= x.tile_rows;
+    x.by_tile_rows = FastDiv::of(x.tile_rows);
+    x.by_G = FastDiv::of(G);
+    x.by_ctas = FastDiv::of(sms);
     x.splits = reinterpret_cast<SplitItem*>(at + (size_t)sms * 2 * rows * (D + 2) * sizeof(float));
     if (tc) return launch_paged_tc(D, f16, qmap, kmap, vmap, x, sms, c.stream);
-    return launch_kernel(D, f16, tokens * G <= 8 ? 1 : tokens * G <= 16 ? 2 : 4, kmap, vmap, x, sms, c.stream);
+    return launch_kernel(D, f16, R / 8, kmap, vmap, x, sms, c.stream);
   };
-  float* state = nullptr;
+  a.table = kv.block_table, a.table_stride = kv.table_stride, a.table_width = kv.table_width;
+  a.r = {c.cu, c.lengths, (int)c.B, (int)c.T, (int)(c.T / c.B)};
+  a.fixed_len = -1, a.cap = kv.table_width * kv.page_size, a.causal = c.causal;
   if (prefix) {
-    // All tokens as one sequence over the prefix, each row seeing all of it.
+    // First each sequence's own keys, into a state per row; then all tokens as
+    // one sequence over the prefix, each row seeing all of it and taking up its
+    // state at the end (so the second launch need not wait for the first).
     char* at = ws + pieces_bytes(most, G, D, sms);
-    state = reinterpret_cast<float*>(at + pieces_bytes(c.T, G, D, sms));
+    float* state = reinterpret_cast<float*>(at + pieces_bytes(c.T, G, D, sms));
+    a.state_acc = state, a.state_ml = state + c.T * c.Hq * D;
+    e = launch(a, ws, most);
     PagedArgs p = a;
     p.table = c.prefix_table, p.table_stride = 0, p.table_width = (int)c.prefix_width;
     p.r = {nullptr, nullptr, 1, (int)c.T, (int)c.T};
     p.fixed_len = (int)c.prefix_len, p.cap = (int)c.prefix_len, p.causal = 0;
-    p.state_acc = state, p.state_ml = state + c.T * c.Hq * D;
-    e = launch(p, at, c.T);
-  }
-  if (e == cudaSuccess) {
-    a.table = kv.block_table, a.table_stride = kv.table_stride, a.table_width = kv.table_width;
-    a.r = {c.cu, c.lengths, (int)c.B, (int)c.T, (int)(c.T / c.B)};
-    a.fixed_len = -1, a.cap = kv.table_width * kv.page_size, a.causal = c.causal;
-    if (prefix) a.prior_acc = state, a.prior_ml = state + c.T * c.Hq * D;
+    p.prior_acc = a.state_acc, p.prior_ml = a.state_ml, p.late = 1;
+    p.state_acc = p.state_ml = nullptr;
+    if (e == cudaSuccess) e = launch(p, at, c.T);
+  } else {
     e = launch(a, ws, most);
   }
   if (own) scratch_free(own, c.stream);

@@ -22,6 +22,21 @@ namespace qi4 {
 
 constexpr int kBlockKeys = 128;  // keys of a unit
 
+// x / d for 0 <= x < 2^31 as a product and a shift (d set on the host): an
+// integer division costs some 150 cycles of latency, and the work split, which
+// runs before a kernel's first load, would hold ten of them.
+struct FastDiv {
+  unsigned mul, shift;  // mul 0: d = 1
+  static FastDiv of(int64_t d) {
+    if (d <= 1) return {0u, 0u};
+    unsigned log = 0;
+    while ((1ll << log) < d) ++log;
+    // ceil(2^(31 + log) / d) is below 2^32, and exact for x below 2^31.
+    return {(unsigned)(((1ull << (31 + log)) + (unsigned long long)d - 1) / (unsigned long long)d), log - 1};
+  }
+  __device__ __forceinline__ int operator()(int x) const { return mul ? (int)(__umulhi((unsigned)x, mul) >> shift) : x; }
+};
+
 struct PagedArgs {
   const uint16_t* q;
   int64_t q_tok, q_head;  // strides, elements
@@ -33,13 +48,19 @@ struct PagedArgs {
   int fixed_len;  // >= 0: every sequence has this many keys (lengths is not read)
   int Hkv, G, cap;
   int causal;
+  int one_tile;                // no sequence has more rows than a tile (decode steps, drafts): the split is shorter
+  int tile_rows, tile_tokens;  // R rows, or the most whole tokens that R rows hold (0 tokens: a token has more rows)
+  FastDiv by_tile_rows, by_G, by_ctas;  // by_ctas: the launch's CTAs
   float scale_log2;  // scale * log2(e)
   float* ws;         // pieces: two slots per CTA, each R x D sums then R x (max, sum)
   struct SplitItem* splits;  // one per CTA: the item that begins in its run and ends beyond it
-  // Keys that every row has seen already (a shared prefix): per row t * Hq + h
-  // the D weighted sums, and (max, sum of weights); or null.
+  // What another launch found for every row: per row t * Hq + h the D weighted
+  // sums, and (max, sum of weights); or null. `late`: that launch is the one
+  // before this, which waits for it only before it reads the state (all else it
+  // reads is older than the launch before that one).
   const float* prior_acc;
   const float* prior_ml;
+  int late;
   // Non-null: the rows' state is written here instead of `out`.
   float* state_acc;
   float* state_ml;
@@ -57,11 +78,21 @@ struct SplitItem {
 // nothing needs a 64-bit division.
 struct Runs {
   int U, C, quot, rest;
+  FastDiv by_C;
   __device__ __forceinline__ Runs() {}
-  __device__ __forceinline__ Runs(int units, int ctas) : U(units), C(ctas), quot(units / ctas), rest(units - quot * ctas) {}
-  __device__ __forceinline__ int start(int c) const { return c * quot + (int)((unsigned)(c * rest) / (unsigned)C); }
+  __device__ __forceinline__ Runs(const PagedArgs& a, int units, int ctas) : U(units), C(min(ctas, units)) {
+    if (units < ctas) {
+      quot = 1, rest = 0;  // one unit each
+      by_C = {0u, 0u};
+    } else {
+      by_C = a.by_ctas;
+      quot = by_C(units);
+      rest = units - quot * ctas;
+    }
+  }
+  __device__ __forceinline__ int start(int c) const { return c * quot + by_C(c * rest); }
   __device__ __forceinline__ int holder(int u) const {  // the CTA that owns unit u
-    int c = min(C - 1, (int)((float)u * ((float)C / (float)U)));
+    int c = min(C - 1, (int)(__fdividef((float)u, (float)U) * (float)C));
     while (start(c) > u) --c;
     while (c + 1 < C && start(c + 1) <= u) ++c;
     return c;
@@ -78,47 +109,52 @@ template <int R>
 struct Walk {
   Runs runs;
   int u, end, item0;  // u: next unit; item0: the current item's first (fixed-cost) unit
-  int tile_rows, tile_tokens;
-  unsigned g_inv;     // ceil(2^16 / G): r / G = r g_inv >> 16 for r, G up to 256
   int b, first, n, len, tiles;       // sequence b: first token, tokens, keys, row tiles
   int tile, kvh, blocks, at;         // item; at: next of its 1 + blocks units
   int blk, nblk;                     // this piece: blocks [blk, blk + nblk) of the item
 
   __device__ __forceinline__ void load(const PagedArgs& a, int seq) {
+    set(a, seq, seq_tokens(a.r, seq), a.fixed_len >= 0 ? a.fixed_len : __ldg(a.r.lengths + seq));
+  }
+  __device__ __forceinline__ void set(const PagedArgs& a, int seq, Tokens t, int length) {
     b = seq;
-    const Tokens t = seq_tokens(a.r, seq);
     first = t.first;
     n = t.count;
-    len = a.fixed_len >= 0 ? a.fixed_len : __ldg(a.r.lengths + seq);
-    len = min(max(len, 0), a.cap);
-    tiles = (n * a.G + tile_rows - 1) / tile_rows;
+    len = min(max(length, 0), a.cap);
+    tiles = a.one_tile ? n > 0 : a.by_tile_rows(n * a.G + a.tile_rows - 1);
   }
   // Keys that tile t's last row sees: none beyond is loaded.
   __device__ __forceinline__ int tile_visible(const PagedArgs& a, int t) const {
-    if (!a.causal) return len;
-    const int last = a.G <= R ? min(n, (t + 1) * tile_tokens) - 1 : (min(n * a.G, (t + 1) * tile_rows) - 1) / a.G;
+    if (!a.causal || a.one_tile) return len;
+    const int last = a.G <= R ? min(n, (t + 1) * a.tile_tokens) - 1 : a.by_G(min(n * a.G, (t + 1) * a.tile_rows) - 1);
     return max(0, min(len, len - n + last + 1));
   }
   __device__ __forceinline__ int tile_visible(const PagedArgs& a) const { return tile_visible(a, tile); }
   __device__ __forceinline__ int blocks_of(const PagedArgs& a, int t) const {
     return max(1, (tile_visible(a, t) + kBlockKeys - 1) / kBlockKeys);
   }
-  // Units of sequences b0 .. b0 + per - 1, one per group of 32 / per lanes (per
-  // a power of two), each lane summing every (32 / per)-th tile; the sum of a
-  // sequence ends up in the first lane of its group, 0 in the others.
-  __device__ __forceinline__ int group_units(const PagedArgs& a, int b0, int per, int lane) {
-    const int lanes = 32 / per, seq = b0 + lane / lanes, sub = lane % lanes;
+  // Units of the loaded sequence, the tiles from `sub` on in steps of `step`.
+  __device__ __forceinline__ int seq_units(const PagedArgs& a, int sub, int step) const {
+    if (!a.causal || a.one_tile) return sub == 0 ? a.Hkv * tiles * (1 + blocks_of(a, 0)) : 0;
     int sum = 0;
-    if (seq < a.r.B) {
-      load(a, seq);
-      if (!a.causal) {
-        if (sub == 0) sum = tiles * (1 + blocks_of(a, 0));
-      } else {
-        for (int t = sub; t < tiles; t += lanes) sum += 1 + blocks_of(a, t);
-      }
+    for (int t = sub; t < tiles; t += step) sum += 1 + blocks_of(a, t);
+    return a.Hkv * sum;
+  }
+  // Units of sequences b0 .. b0 + 3, all their loads before the first use.
+  __device__ __forceinline__ void quad_units(const PagedArgs& a, int b0, int (&w)[4]) {
+    Tokens t[4];
+    int l[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int seq = min(b0 + i, a.r.B - 1);
+      t[i] = seq_tokens(a.r, seq);
+      l[i] = a.fixed_len >= 0 ? a.fixed_len : __ldg(a.r.lengths + seq);
     }
-    for (int o = lanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    return sub == 0 ? sum * a.Hkv : 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      set(a, b0 + i, t[i], l[i]);
+      w[i] = b0 + i < a.r.B ? seq_units(a, 0, 1) : 0;
+    }
   }
   static __device__ __forceinline__ int scan(int x, int lane) {
 #pragma unroll
@@ -130,34 +166,55 @@ struct Walk {
   }
   // False if the CTA has no units.
   __device__ __forceinline__ bool begin(const PagedArgs& a, int lane) {
-    tile_tokens = R / a.G;  // 0 where a token has more rows than a tile
-    tile_rows = a.G <= R ? tile_tokens * a.G : R;
-    int per = 32;
-    while (per > 1 && per / 2 >= a.r.B) per >>= 1;
-    g_inv = (65535u + a.G) / (unsigned)a.G;
-    int U = 0, mine = 0;
-    for (int b0 = 0; b0 < a.r.B; b0 += per) {
-      mine = group_units(a, b0, per, lane);
-      U += __reduce_add_sync(0xffffffffu, mine);
-    }
-    const int C = min((int)gridDim.x, U);
-    if ((int)blockIdx.x >= C) return false;
-    runs = Runs(U, C);
-    u = runs.start(blockIdx.x);
-    end = runs.start(blockIdx.x + 1);
-    // The sequence that holds unit u, then the tile.
-    int before = 0, seq = 0;
-    for (int b0 = 0; b0 < a.r.B; b0 += per) {
-      if (a.r.B > per) mine = group_units(a, b0, per, lane);
-      const int incl = scan(mine, lane);
-      const unsigned hit = __ballot_sync(0xffffffffu, before + incl > u);
-      if (hit) {
-        const int src = __ffs(hit) - 1;
-        seq = b0 + src / (32 / per);
-        before += __shfl_sync(0xffffffffu, incl - mine, src);
-        break;
+    int U = 0, before = 0, seq = 0;
+    if (a.r.B <= 32) {
+      // A sequence for each group of lanes, which share its tiles.
+      int lanes = 32;
+      while (lanes > 1 && 32 / lanes < a.r.B) lanes >>= 1;
+      int mine = 0;
+      if (lane / lanes < a.r.B) {
+        load(a, lane / lanes);
+        mine = seq_units(a, lane & (lanes - 1), lanes);
       }
-      before += __shfl_sync(0xffffffffu, incl, 31);
+      for (int o = lanes / 2; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+      if (lane & (lanes - 1)) mine = 0;
+      const int incl = scan(mine, lane);
+      U = __shfl_sync(0xffffffffu, incl, 31);
+      if (!deal(a, U)) return false;
+      const unsigned hit = __ballot_sync(0xffffffffu, incl > u);
+      const int src = __ffs(hit) - 1;
+      seq = src / lanes;
+      before = __shfl_sync(0xffffffffu, incl - mine, src);
+    } else {
+      // 128 at a time, four in a row for each lane; the first 128 stay at hand for the second pass.
+      int kept[4];
+      quad_units(a, 4 * lane, kept);
+      U = __reduce_add_sync(0xffffffffu, kept[0] + kept[1] + kept[2] + kept[3]);
+      for (int b0 = 128; b0 < a.r.B; b0 += 128) {
+        int more[4];
+        quad_units(a, b0 + 4 * lane, more);
+        U += __reduce_add_sync(0xffffffffu, more[0] + more[1] + more[2] + more[3]);
+      }
+      if (!deal(a, U)) return false;
+      for (int b0 = 0; b0 < a.r.B; b0 += 128) {
+        if (b0) quad_units(a, b0 + 4 * lane, kept);
+        const int mine = kept[0] + kept[1] + kept[2] + kept[3], incl = scan(mine, lane);
+        const unsigned hit = __ballot_sync(0xffffffffu, before + incl > u);
+        if (hit) {
+          int at0 = before + incl - mine, i = 0;
+#pragma unroll
+          for (int k = 0; k < 3; ++k)
+            if (i == k && at0 + kept[k] <= u) {
+              at0 += kept[k];
+              ++i;
+            }
+          const int src = __ffs(hit) - 1;
+          seq = __shfl_sync(0xffffffffu, b0 + 4 * lane + i, src);
+          before = __shfl_sync(0xffffffffu, at0, src);
+          break;
+        }
+        before += __shfl_sync(0xffffffffu, incl, 31);
+      }
     }
     load(a, seq);
     for (tile = 0; tile + 1 < tiles; tile += 32) {
@@ -174,8 +231,18 @@ struct Walk {
     }
     blocks = blocks_of(a, tile);
     at = u - before;
-    kvh = at / (1 + blocks);
+    kvh = min(a.Hkv - 1, (int)__fdividef((float)at, (float)(1 + blocks)));
+    while (kvh * (1 + blocks) > at) --kvh;
+    while ((kvh + 1) * (1 + blocks) <= at) ++kvh;
     at -= kvh * (1 + blocks);
+    return true;
+  }
+  // This CTA's run of U units.
+  __device__ __forceinline__ bool deal(const PagedArgs& a, int U) {
+    if ((int)blockIdx.x >= min((int)gridDim.x, U)) return false;
+    runs = Runs(a, U, gridDim.x);
+    u = runs.start(blockIdx.x);
+    end = runs.start(blockIdx.x + 1);
     return true;
   }
   // The next piece; false behind the last.
@@ -206,23 +273,16 @@ struct Walk {
     }
   }
   __device__ __forceinline__ bool whole() const { return nblk == blocks; }
-  __device__ __forceinline__ int rows(const PagedArgs& a) const { return min(tile_rows, n * a.G - tile * tile_rows); }
-  __device__ __forceinline__ int row0() const { return tile * tile_rows; }
+  __device__ __forceinline__ int rows(const PagedArgs& a) const { return min(a.tile_rows, n * a.G - tile * a.tile_rows); }
+  __device__ __forceinline__ int row0(const PagedArgs& a) const { return tile * a.tile_rows; }
   // Token and query head of row r of the tile.
   __device__ __forceinline__ void place(const PagedArgs& a, int r, int& token, int& head) const {
-    if (a.G <= R) {
-      const int t = (int)(r * g_inv >> 16);
-      token = first + tile * tile_tokens + t;
-      head = kvh * a.G + r - t * a.G;
-    } else {
-      const int t = (row0() + r) / a.G;
-      token = first + t;
-      head = kvh * a.G + row0() + r - t * a.G;
-    }
+    const int row = row0(a) + r, t = a.by_G(row);
+    token = first + t;
+    head = kvh * a.G + row - t * a.G;
   }
   __device__ __forceinline__ int row_visible(const PagedArgs& a, int r) const {
-    const int t = a.G <= R ? tile * tile_tokens + (int)(r * g_inv >> 16) : (row0() + r) / a.G;
-    return a.causal ? max(0, min(len, len - n + t + 1)) : len;
+    return a.causal ? max(0, min(len, len - n + a.by_G(row0(a) + r) + 1)) : len;
   }
   // Blocks of this piece that hold visible keys: all, but for an item of one empty block.
   __device__ __forceinline__ int loaded(int vis) const { return vis > 0 ? nblk : 0; }
@@ -294,7 +354,7 @@ template <int R>
 __device__ __forceinline__ void note_split(const PagedArgs& a, const Walk<R>& w, bool any) {
   SplitItem it = {0, 0, 0, 0, 0, 0};
   if (any && w.blk == 0 && w.nblk > 0 && !w.whole())
-    it = {w.pieces(), w.slot(blockIdx.x), w.rows(a), w.first, w.row0(), w.kvh};
+    it = {w.pieces(), w.slot(blockIdx.x), w.rows(a), w.first, w.row0(a), w.kvh};
   a.splits[blockIdx.x] = it;
 }
 

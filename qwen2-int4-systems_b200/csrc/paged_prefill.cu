@@ -32,6 +32,7 @@
 // a product of N = 64 with both operands in shared memory takes the 64 cycles
 // of one with N = 128.)
 // Tensor memory: scores 2 x 128 columns, sums 2 x D. All waits are bounded.
+#include <algorithm>
 #include <atomic>
 
 #include "paged_attention.cuh"
@@ -185,7 +186,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;  // S0, S1 at 0, 128; O0, O1 at 256, 256 + D
-  pdl_wait();
+  if (!a.late) pdl_wait();
   pdl_launch_dependents();
 
   Walk<kTcRows> w;
@@ -202,15 +203,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         // sequence that come with a sequence's last tile, and rows past the box, only make rows that nobody reads.
         mbar_wait(q_empty, (nq++ & 1u) ^ 1u, &g_paged_tc_error);
         if (lane == 0) {
-          mbar_arrive_expect_tx(q_full, (uint32_t)(w.tile_rows * D * 2));
+          mbar_arrive_expect_tx(q_full, (uint32_t)(a.tile_rows * D * 2));
 #pragma unroll
           for (int h = 0; h < D / 64; ++h)
-            tma_load_3d(q_s + h * kQHalf, &qmap, 64 * h, w.kvh * a.G, w.first + w.tile * w.tile_tokens, q_full);
+            tma_load_3d(q_s + h * kQHalf, &qmap, 64 * h, w.kvh * a.G, w.first + w.tile * a.tile_tokens, q_full);
         }
         __syncwarp();
       }
       if (lane == 0 && a.fixed_len < 0 && __ldg(a.r.lengths + w.b) > a.cap)
         atomicOr(&g_paged_tc_error, kErrCacheFull);
+      if (lane == 0 && a.one_tile && w.n * a.G > a.tile_rows)
+        atomicOr(&g_paged_tc_error, QI4_DEVICE_TOO_MANY_TOKENS);
       int win0 = -1, win = -1;
       for (int i = 0; i < w.nblk; ++i) {
         const int key0 = (w.blk + i) * kBlockKeys;
@@ -238,6 +241,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
+    if (lane == 0) note_split(a, w, true);
   } else if (any && warp == kSoftmaxWarps) {
     // ---- products ----
     // The whole warp runs the loops and the waits; one lane issues.
@@ -404,6 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&p_full[2 * t + x]);
       }
       have = w.next(a);
+      if (a.late) pdl_wait();
       if (nload > 0) {
         done += 2 * nload;
         mbar_wait(&o_full[t], no++ & 1u, &g_paged_tc_error);
@@ -432,8 +437,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (live && !whole) *reinterpret_cast<float2*>(slot + kTcRows * D + 2 * row) = make_float2(m, l);
       tc_fence_before();  // the sums are read before the next item's first weights are announced
     }
-    if (threadIdx.x == 0) note_split(a, w, any);
   }
+  if (!any && threadIdx.x == 0) note_split(a, w, false);
   tc_fence_before();
   __syncthreads();
   if (warp == kSoftmaxWarps) {
@@ -445,78 +450,74 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // Joins the pieces of the item that begins in CTA blockIdx.x's run and ends
 // beyond it, if there is one: block (c, y, z) takes 32 rows and 32 dims. A
-// piece is [D][kTcRows] sums, then [kTcRows] (max, sum): lanes are rows.
-constexpr int kJoinThreads = 256, kMaxPieces = 160;  // at most one piece per CTA
+// piece is [D][kTcRows] sums, then [kTcRows] (max, sum): lanes are rows, eight
+// pieces' loads under way at once.
+constexpr int kJoinThreads = 256;
 template <int D, bool F16>
 __global__ void __launch_bounds__(kJoinThreads) paged_tc_join_kernel(const PagedArgs a) {
   constexpr int64_t kSlot = (int64_t)kTcRows * (D + 2);
-  __shared__ float f_s[kMaxPieces][32];  // max, then weight of piece p for a row
-  __shared__ float l_s[kMaxPieces][32];
-  __shared__ float out_s[32][33];
-  pdl_wait();
+  constexpr int kAtOnce = 8;
+  __shared__ float out_s[32][33], top_s[32], l_s[32];
   pdl_launch_dependents();
+  pdl_wait();
   const SplitItem it = a.splits[blockIdx.x];
   const int r0 = 32 * blockIdx.y, np = it.pieces;
   if (r0 >= it.rows) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = r0 + lane;
+  const int d0 = 4 * warp, d = 32 * blockIdx.z + d0;
   const float* first = a.ws + it.slot * kSlot;
   const float* later = a.ws + 2 * (int64_t)blockIdx.x * kSlot;
-  for (int p = warp; p < np; p += 8) {
-    const float2 ml =
-        *reinterpret_cast<const float2*>((p ? later + 2 * p * kSlot : first) + (int64_t)kTcRows * D + 2 * r);
-    f_s[p][lane] = ml.x;
-    l_s[p][lane] = ml.y;
-  }
-  __syncthreads();
-  float top = -INFINITY;
-  for (int p = 0; p < np; ++p) top = fmaxf(top, f_s[p][lane]);
-  __syncthreads();
-  const float base = top == -INFINITY ? 0.f : top;
-  for (int p = warp; p < np; p += 8) f_s[p][lane] = exp2_approx(f_s[p][lane] - base);
-  __syncthreads();
-  const int d0 = 4 * warp, d = 32 * blockIdx.z + d0;
-  float acc[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
-  for (int p0 = 0; p0 < np; p0 += 4) {
-    float v[4][4], f[4];
+  float acc[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f, top = -INFINITY;
+  for (int p0 = 0; p0 < np; p0 += kAtOnce) {
+    float v[kAtOnce][4];
+    float2 ml[kAtOnce];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kAtOnce; ++i) {
       const int p = p0 + i;
-      f[i] = 0.f;
+      ml[i] = make_float2(-INFINITY, 0.f);
 #pragma unroll
       for (int k = 0; k < 4; ++k) v[i][k] = 0.f;
       if (p < np) {
-        const float* src = (p ? later + 2 * p * kSlot : first) + (int64_t)d * kTcRows + r;
+        const float* src = p ? later + 2 * p * kSlot : first;
+        ml[i] = *reinterpret_cast<const float2*>(src + (int64_t)kTcRows * D + 2 * r);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[i][k] = src[k * kTcRows];
-        f[i] = f_s[p][lane];
-        l += l_s[p][lane] * f[i];
+        for (int k = 0; k < 4; ++k) v[i][k] = src[(d + k) * kTcRows + r];
       }
     }
+    float to = top;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < kAtOnce; ++i) to = fmaxf(to, ml[i].x);
+    const float base = to == -INFINITY ? 0.f : to, back = exp2_approx(top - base);
+    top = to;
+    l *= back;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) acc[k] += v[i][k] * f[i];
+    for (int k = 0; k < 4; ++k) acc[k] *= back;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const float f = exp2_approx(ml[i].x - base);
+      l += ml[i].y * f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[k] += v[i][k] * f;
+    }
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k) out_s[lane][d0 + k] = acc[k];
-  __syncthreads();  // (every warp is through with the weights, too)
-  if (warp == 0) f_s[0][lane] = top, l_s[0][lane] = l;
+  if (warp == 0) top_s[lane] = top, l_s[lane] = l;
   __syncthreads();
   const int orow = threadIdx.x / 8, od = (threadIdx.x % 8) * 4;
   if (r0 + orow < it.rows) {
     float x[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) x[k] = out_s[orow][od + k];
-    const int row = it.row0 + r0 + orow, token = row / a.G;
-    finish_row<D, F16, 4>(a, it.first + token, it.kvh * a.G + row - token * a.G, 32 * blockIdx.z + od, x,
-                          f_s[0][orow], l_s[0][orow]);
+    const int row = it.row0 + r0 + orow, token = a.by_G(row);
+    finish_row<D, F16, 4>(a, it.first + token, it.kvh * a.G + row - token * a.G, 32 * blockIdx.z + od, x, top_s[orow],
+                          l_s[orow]);
   }
 }
 
 template <int D, bool F16>
-cudaError_t launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const PagedArgs& a, int sms,
+cudaError_t launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const PagedArgs& a, int ctas,
                    cudaStream_t s) {
-  const int ctas = sms < kMaxPieces ? sms : kMaxPieces;
   auto kernel = paged_tc_kernel<D, F16>;
   static std::atomic<unsigned long long> configured{0};
   int dev = 0;
@@ -539,7 +540,9 @@ cudaError_t launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap
   cfg.numAttrs = 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, q, k, v, a);
   if (e != cudaSuccess) return e;
-  cfg.gridDim = dim3((unsigned)ctas, kTcRows / 32, D / 32);
+  // (No tile has more rows than the whole batch.)
+  const int64_t rows = std::min<int64_t>(a.tile_rows, (int64_t)a.r.T * a.G);
+  cfg.gridDim = dim3((unsigned)ctas, (unsigned)((rows + 31) / 32), D / 32);
   cfg.blockDim = dim3(kJoinThreads, 1, 1);
   cfg.dynamicSmemBytes = 0;
   return cudaLaunchKernelEx(&cfg, paged_tc_join_kernel<D, F16>, a);

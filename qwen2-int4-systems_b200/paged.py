@@ -68,8 +68,9 @@ def b200_paged_attention(q, k_cache, v_cache, block_table, lengths, *, cu_tokens
     lengths [B]: the sequences' keys, the new tokens' included. Causal: token
     i of a sequence's n sees the keys up to position lengths[b] - n + i; else
     all of them. A token that sees no key gets zeros. ``max_tokens`` (a host
-    number: no sequence has more new tokens) lets a batch given by
-    ``cu_tokens`` run on the kernel for its row count. ``workspace``: a uint8
+    number: no sequence has more new tokens, which ``qi4_device_status``
+    checks) lets a batch given by ``cu_tokens`` run on the kernel and the
+    tiles for its row count. ``workspace``: a uint8
     tensor of ``qi4_paged_attention_workspace`` bytes, for callers that own
     their memory.
     """

@@ -158,6 +158,9 @@ def test_lengths_and_pages_that_do_not_fit_are_reported(b200, cuda_device):
     assert torch.count_nonzero(none) == 0 and _status(b200) == 0
     wild = torch.tensor([-4, 10 ** 8, 10 ** 9], dtype=torch.int32, device=cuda_device)
     b200.b200_paged_attention(x["q"], x["k"], x["v"], x["table"], x["lengths"], cu_tokens=wild)
+    y = pg.build([(9, 100), (12, 30)], Hq=4, Hkv=2, D=64, page=16, dtype=BF16, device=cuda_device)
+    _run(b200, y, max_tokens=4)
+    assert _status(b200) == 32
     empty = b200.b200_paged_attention(x["q"][:0], x["k"], x["v"], x["table"], x["lengths"])
     assert empty.shape == (0, 4, 64) and _status(b200) == 0
 
