@@ -35,6 +35,21 @@ __device__ __forceinline__ Tokens seq_tokens(const Ragged& r, int b) {
   return {t0, t1 - t0};
 }
 
+// x / d for 0 <= x < 2^31 as a product and a shift (d set on the host): an
+// integer division costs some 150 cycles of latency, and the work split, which
+// runs before a kernel's first load, would hold ten of them.
+struct FastDiv {
+  unsigned mul, shift;  // mul 0: d = 1
+  static FastDiv of(int64_t d) {
+    if (d <= 1) return {0u, 0u};
+    unsigned log = 0;
+    while ((1ll << log) < d) ++log;
+    // ceil(2^(31 + log) / d) is below 2^32, and exact for x below 2^31.
+    return {(unsigned)(((1ull << (31 + log)) + (unsigned long long)d - 1) / (unsigned long long)d), log - 1};
+  }
+  __device__ __forceinline__ int operator()(int x) const { return mul ? (int)(__umulhi((unsigned)x, mul) >> shift) : x; }
+};
+
 // Device-side error bits of the paged operators (read by qi4_device_status).
 constexpr int kErrCacheFull = QI4_DEVICE_CACHE_FULL;
 constexpr int kErrBadPage = QI4_DEVICE_BAD_PAGE;

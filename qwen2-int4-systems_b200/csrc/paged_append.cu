@@ -8,13 +8,15 @@
 // are FP32 and each result is rounded once to the cache's type. The key and
 // the value go to slot p % page_size of page block_table[b][p / page_size].
 //
-// A thread owns one unit: 16 dimensions of one head of one token, as two
-// 16-byte chunks that hold whole pairs (the chunks m and m + rot/2 of 8
-// dimensions each, or two adjacent chunks), so that both layouts read the
-// same 8 cosines and sines and no value passes between threads. Bound by
-// memory (each byte is read and written once); the loads of a thread's units
-// are issued before the chain sequence -> length -> page that finds where
-// they go, which is three dependent loads and the whole time of a small call.
+// A thread owns one unit at a time: 16 dimensions of one head of one token, as
+// two 16-byte chunks that hold whole pairs (the chunks m and m + rot/2 of 8
+// dimensions each, or two adjacent chunks), so that both layouts read the same
+// 8 cosines and sines and no value passes between threads. Bound by memory
+// (each byte is read and written once). A CTA owns up to 64 tokens; one thread
+// per token follows the chain boundaries -> sequence -> length -> page that
+// says where it goes, three dependent loads, once per CTA and behind the first
+// two units' loads of every thread; from there each thread has the loads of
+// two units ahead of it under way.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -47,6 +49,7 @@ struct AppendArgs {
   int rope_rows, rot_units, half;  // rot / 16, rot / 2
   int Hq, Hkv, units_per_head;     // D / 16
   int tokens_per_cta;
+  FastDiv by_units, by_head, by_per_seq;
   int interleaved;
 };
 
@@ -79,124 +82,139 @@ __device__ __forceinline__ uint4 pack(const float (&x)[8]) {
   return make_uint4(a[0], a[1], a[2], a[3]);
 }
 
-// The sequence of token t: the number of sequences that end at or before it
-// (empty ones are passed over), counted by the warp 32 boundaries at a time.
-__device__ __forceinline__ int owner_of(const Ragged& r, int t, int lane) {
-  if (!r.cu) return t / r.per_seq;
-  int before = 0;
-  for (int j = lane; j < r.B; j += 32) before += __ldg(r.cu + j + 1) <= t;
-  return __reduce_add_sync(0xffffffffu, before);
+// The sequence of token t (the number of sequences that end at or before it,
+// so that empty ones are passed over), or -1 where no sequence has it.
+__device__ __forceinline__ int owner_of(const Ragged& r, const FastDiv& by_per_seq, int t) {
+  if (!r.cu) return by_per_seq(t);
+  int lo = 0, hi = r.B;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (__ldg(r.cu + mid + 1) <= t)
+      lo = mid + 1;
+    else
+      hi = mid;
+  }
+  if (lo >= r.B) return -1;
+  const Tokens s = seq_tokens(r, lo);
+  return t >= s.first && t < s.first + s.count ? lo : -1;
 }
 
-// ITER units per thread in flight.
-template <bool F16, int ITER>
-__global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
+struct Unit {
+  int64_t t;
+  int tk, h, c0, c1;  // token of the CTA, head (q, then k, then v), the two chunks' dimensions
+  bool turned;
+  int u;
+};
+
+template <bool F16>
+__global__ void __launch_bounds__(kThreads, 4) append_kernel(const AppendArgs a) {
   __shared__ int64_t slot_of[kMaxTokens];  // element offset of the token's slot in the pool, or -1
   __shared__ int row_of[kMaxTokens];       // row of cos / sin
   pdl_wait();
   pdl_launch_dependents();
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int heads = a.Hq + 2 * a.Hkv, units = heads * a.units_per_head;
+  const int tid = threadIdx.x;
+  const int units = (a.Hq + 2 * a.Hkv) * a.units_per_head;
   const int t0 = blockIdx.x * a.tokens_per_cta;
   const int nt = min(a.tokens_per_cta, a.r.T - t0);
   const int total = nt * units;
 
-  for (int base = 0; base < total; base += kThreads * ITER) {
-    uint4 lo[ITER], hi[ITER];
+  auto unit = [&](int idx) {
+    Unit x;
+    x.tk = a.by_units(idx);
+    const int rest = idx - x.tk * units;
+    x.h = a.by_head(rest);
+    x.u = rest - x.h * a.units_per_head;
+    x.t = t0 + x.tk;
+    x.turned = x.h < a.Hq + a.Hkv && x.u < a.rot_units;
+    const bool halves = x.turned && !a.interleaved;
+    x.c0 = halves ? 8 * x.u : 16 * x.u;
+    x.c1 = halves ? x.c0 + a.half : x.c0 + 8;
+    return x;
+  };
+  auto fetch = [&](int idx, uint4& lo, uint4& hi) {
+    if (idx >= total) return;
+    const Unit x = unit(idx);
+    const uint16_t* src = x.h < a.Hq ? a.q + x.t * a.q_tok + x.h * a.q_head
+                          : x.h < a.Hq + a.Hkv ? a.k + x.t * a.k_tok + (x.h - a.Hq) * a.k_head
+                                               : a.v + x.t * a.v_tok + (x.h - a.Hq - a.Hkv) * a.v_head;
+    lo = *reinterpret_cast<const uint4*>(src + x.c0);
+    hi = *reinterpret_cast<const uint4*>(src + x.c1);
+  };
+  auto place = [&](int idx, uint4 w0, uint4 w1) {
+    if (idx >= total) return;
+    const Unit x = unit(idx);
+    if (x.turned) {
+      const float4* cp = reinterpret_cast<const float4*>(a.cos + (int64_t)row_of[x.tk] * a.half + 8 * x.u);
+      const float4* sp = reinterpret_cast<const float4*>(a.sin + (int64_t)row_of[x.tk] * a.half + 8 * x.u);
+      const float4 ca = __ldg(cp), cb = __ldg(cp + 1), sa = __ldg(sp), sb = __ldg(sp + 1);
+      const float c[8] = {ca.x, ca.y, ca.z, ca.w, cb.x, cb.y, cb.z, cb.w};
+      const float s[8] = {sa.x, sa.y, sa.z, sa.w, sb.x, sb.y, sb.z, sb.w};
+      float e[8], f[8], re[8], rf[8];
+      unpack<F16>(w0, e);
+      unpack<F16>(w1, f);
+      if (a.interleaved) {
 #pragma unroll
-    for (int i = 0; i < ITER; ++i) {
-      const int idx = base + i * kThreads + tid;
-      if (idx >= total) break;
-      const int tk = idx / units, rest = idx - tk * units, h = rest / a.units_per_head,
-                u = rest - h * a.units_per_head;
-      const int64_t t = t0 + tk;
-      const uint16_t* src = h < a.Hq ? a.q + t * a.q_tok + h * a.q_head
-                            : h < a.Hq + a.Hkv ? a.k + t * a.k_tok + (h - a.Hq) * a.k_head
-                                               : a.v + t * a.v_tok + (h - a.Hq - a.Hkv) * a.v_head;
-      const bool halves = h < a.Hq + a.Hkv && u < a.rot_units && !a.interleaved;
-      const int c0 = halves ? 8 * u : 16 * u, c1 = halves ? c0 + a.half : c0 + 8;
-      lo[i] = *reinterpret_cast<const uint4*>(src + c0);
-      hi[i] = *reinterpret_cast<const uint4*>(src + c1);
-    }
-    if (base == 0) {  // where the CTA's tokens go, one warp per token at a time
-      for (int j = warp; j < nt; j += kThreads / 32) {
-        const int t = t0 + j;
-        const int b = owner_of(a.r, t, lane);
-        if (lane == 0) {
-          int64_t slot = -1;
-          int row = 0;
-          if (b < a.r.B) {
-            const Tokens s = seq_tokens(a.r, b);
-            const int64_t at = (int64_t)__ldg(a.r.lengths + b) + (t - s.first);
-            const int64_t pj = at >> a.page_shift;
-            if (at < 0 || pj >= a.table_width) {
-              atomicOr(&g_append_error, kErrCacheFull);
-            } else {
-              const int page = __ldg(a.table + b * a.table_stride + pj);
-              if (page < 0 || page >= a.pages)
-                atomicOr(&g_append_error, kErrBadPage);
-              else
-                slot = (int64_t)page * a.page_stride + (at & (a.page_size - 1)) * a.slot_stride;
-            }
-            const int64_t want = a.positions ? (int64_t)__ldg(a.positions + t) : at;
-            row = (int)max((int64_t)0, min(want, (int64_t)a.rope_rows - 1));
-            if (want != row && a.rot_units) atomicOr(&g_append_error, kErrBadPosition);
-          }
-          slot_of[j] = slot;
-          row_of[j] = row;
+        for (int m = 0; m < 4; ++m) {
+          re[2 * m] = e[2 * m] * c[m] - e[2 * m + 1] * s[m];
+          re[2 * m + 1] = e[2 * m + 1] * c[m] + e[2 * m] * s[m];
+          rf[2 * m] = f[2 * m] * c[m + 4] - f[2 * m + 1] * s[m + 4];
+          rf[2 * m + 1] = f[2 * m + 1] * c[m + 4] + f[2 * m] * s[m + 4];
         }
-      }
-      __syncthreads();
-    }
-#pragma unroll
-    for (int i = 0; i < ITER; ++i) {
-      const int idx = base + i * kThreads + tid;
-      if (idx >= total) break;
-      const int tk = idx / units, rest = idx - tk * units, h = rest / a.units_per_head,
-                u = rest - h * a.units_per_head;
-      const int64_t t = t0 + tk;
-      const bool turned = h < a.Hq + a.Hkv && u < a.rot_units;
-      const bool halves = turned && !a.interleaved;
-      const int c0 = halves ? 8 * u : 16 * u, c1 = halves ? c0 + a.half : c0 + 8;
-      uint4 w0 = lo[i], w1 = hi[i];
-      if (turned) {
-        const float4* cp = reinterpret_cast<const float4*>(a.cos + (int64_t)row_of[tk] * a.half + 8 * u);
-        const float4* sp = reinterpret_cast<const float4*>(a.sin + (int64_t)row_of[tk] * a.half + 8 * u);
-        const float4 ca = __ldg(cp), cb = __ldg(cp + 1), sa = __ldg(sp), sb = __ldg(sp + 1);
-        const float c[8] = {ca.x, ca.y, ca.z, ca.w, cb.x, cb.y, cb.z, cb.w};
-        const float s[8] = {sa.x, sa.y, sa.z, sa.w, sb.x, sb.y, sb.z, sb.w};
-        float x[8], y[8], rx[8], ry[8];
-        unpack<F16>(w0, x);
-        unpack<F16>(w1, y);
-        if (a.interleaved) {
-#pragma unroll
-          for (int m = 0; m < 4; ++m) {
-            rx[2 * m] = x[2 * m] * c[m] - x[2 * m + 1] * s[m];
-            rx[2 * m + 1] = x[2 * m + 1] * c[m] + x[2 * m] * s[m];
-            ry[2 * m] = y[2 * m] * c[m + 4] - y[2 * m + 1] * s[m + 4];
-            ry[2 * m + 1] = y[2 * m + 1] * c[m + 4] + y[2 * m] * s[m + 4];
-          }
-        } else {
-#pragma unroll
-          for (int m = 0; m < 8; ++m) {
-            rx[m] = x[m] * c[m] - y[m] * s[m];
-            ry[m] = y[m] * c[m] + x[m] * s[m];
-          }
-        }
-        w0 = pack<F16>(rx);
-        w1 = pack<F16>(ry);
-      }
-      uint16_t* dst;
-      if (h < a.Hq) {
-        dst = a.q_out + t * a.o_tok + h * a.o_head;
       } else {
-        if (slot_of[tk] < 0) continue;
-        const bool key = h < a.Hq + a.Hkv;
-        dst = (key ? a.k_pages : a.v_pages) + slot_of[tk] +
-              (int64_t)(h - a.Hq - (key ? 0 : a.Hkv)) * a.head_stride;
+#pragma unroll
+        for (int m = 0; m < 8; ++m) {
+          re[m] = e[m] * c[m] - f[m] * s[m];
+          rf[m] = f[m] * c[m] + e[m] * s[m];
+        }
       }
-      *reinterpret_cast<uint4*>(dst + c0) = w0;
-      *reinterpret_cast<uint4*>(dst + c1) = w1;
+      w0 = pack<F16>(re);
+      w1 = pack<F16>(rf);
+    }
+    uint16_t* dst;
+    if (x.h < a.Hq) {
+      dst = a.q_out + x.t * a.o_tok + x.h * a.o_head;
+    } else {
+      if (slot_of[x.tk] < 0) return;
+      const bool key = x.h < a.Hq + a.Hkv;
+      dst = (key ? a.k_pages : a.v_pages) + slot_of[x.tk] + (int64_t)(x.h - a.Hq - (key ? 0 : a.Hkv)) * a.head_stride;
+    }
+    *reinterpret_cast<uint4*>(dst + x.c0) = w0;
+    *reinterpret_cast<uint4*>(dst + x.c1) = w1;
+  };
+
+  uint4 lo[2], hi[2];
+  fetch(tid, lo[0], hi[0]);
+  fetch(tid + kThreads, lo[1], hi[1]);
+  if (tid < nt) {
+    const int t = t0 + tid, b = owner_of(a.r, a.by_per_seq, t);
+    int64_t slot = -1;
+    int row = 0;
+    if (b >= 0) {
+      const int64_t at = (int64_t)__ldg(a.r.lengths + b) + (t - seq_tokens(a.r, b).first);
+      const int64_t pj = at >> a.page_shift;
+      if (at < 0 || pj >= a.table_width) {
+        atomicOr(&g_append_error, kErrCacheFull);
+      } else {
+        const int page = __ldg(a.table + b * a.table_stride + pj);
+        if (page < 0 || page >= a.pages)
+          atomicOr(&g_append_error, kErrBadPage);
+        else
+          slot = (int64_t)page * a.page_stride + (at & (a.page_size - 1)) * a.slot_stride;
+      }
+      const int64_t want = a.positions ? (int64_t)__ldg(a.positions + t) : at;
+      row = (int)max((int64_t)0, min(want, (int64_t)a.rope_rows - 1));
+      if (want != row && a.rot_units) atomicOr(&g_append_error, kErrBadPosition);
+    }
+    slot_of[tid] = slot;
+    row_of[tid] = row;
+  }
+  __syncthreads();
+  for (int base = tid; base < total; base += 2 * kThreads) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint4 w0 = lo[i], w1 = hi[i];
+      fetch(base + (i + 2) * kThreads, lo[i], hi[i]);
+      place(base + i * kThreads, w0, w1);
     }
   }
 }
@@ -205,10 +223,16 @@ template <bool F16>
 cudaError_t launch_append(const AppendArgs& a0, int sms, cudaStream_t stream) {
   AppendArgs a = a0;
   const int units = (a.Hq + 2 * a.Hkv) * a.units_per_head;
-  // Two units in flight per thread once the call fills the GPU several times
-  // over, one (the shortest path) below.
-  const bool wide = (int64_t)a.r.T * units > (int64_t)sms * 8 * kThreads;
-  a.tokens_per_cta = std::max(1, std::min(kMaxTokens, kThreads * (wide ? 2 : 1) / units));
+  // Few tokens per CTA while that gives every SM work (the chain above is then
+  // the whole time), six rounds of units once the call fills the GPU: 36,238
+  // tokens of 24 heads x 128 take 88 us with three rounds, 81 with six, 82 with
+  // twelve (454 MB: 5.6 TB/s), 64 decode steps 2.8.
+  const int64_t all = (int64_t)a.r.T * units;
+  const int64_t per_cta = all <= (int64_t)sms * 4 * kThreads ? kThreads : 6 * kThreads;
+  a.tokens_per_cta = (int)std::max<int64_t>(1, std::min<int64_t>(kMaxTokens, per_cta / units));
+  a.by_units = FastDiv::of(units);
+  a.by_head = FastDiv::of(a.units_per_head);
+  a.by_per_seq = FastDiv::of(a.r.per_seq);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -218,7 +242,7 @@ cudaError_t launch_append(const AppendArgs& a0, int sms, cudaStream_t stream) {
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return wide ? cudaLaunchKernelEx(&cfg, append_kernel<F16, 2>, a) : cudaLaunchKernelEx(&cfg, append_kernel<F16, 1>, a);
+  return cudaLaunchKernelEx(&cfg, append_kernel<F16>, a);
 }
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

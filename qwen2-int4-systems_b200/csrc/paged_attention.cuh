@@ -22,21 +22,6 @@ namespace qi4 {
 
 constexpr int kBlockKeys = 128;  // keys of a unit
 
-// x / d for 0 <= x < 2^31 as a product and a shift (d set on the host): an
-// integer division costs some 150 cycles of latency, and the work split, which
-// runs before a kernel's first load, would hold ten of them.
-struct FastDiv {
-  unsigned mul, shift;  // mul 0: d = 1
-  static FastDiv of(int64_t d) {
-    if (d <= 1) return {0u, 0u};
-    unsigned log = 0;
-    while ((1ll << log) < d) ++log;
-    // ceil(2^(31 + log) / d) is below 2^32, and exact for x below 2^31.
-    return {(unsigned)(((1ull << (31 + log)) + (unsigned long long)d - 1) / (unsigned long long)d), log - 1};
-  }
-  __device__ __forceinline__ int operator()(int x) const { return mul ? (int)(__umulhi((unsigned)x, mul) >> shift) : x; }
-};
-
 struct PagedArgs {
   const uint16_t* q;
   int64_t q_tok, q_head;  // strides, elements
