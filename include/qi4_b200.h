@@ -496,7 +496,7 @@ QI4_API size_t qi4_paged_attention_workspace(int64_t T, int64_t Hq, int64_t kv_h
  *   of `dtype` at the given strides (elements), V contiguous; draft_probs NULL:
  *   drafts without a distribution (q = 1 at the token); uniforms [B, K + 1];
  *   out_tokens [B, K + 1]: the standing drafts, the drawn token, then -1;
- *   accepted [B]: a. K <= 4096, V <= 2^22. No reference counterpart.
+ *   accepted [B]: a. K <= 4096, V <= 2^21. No reference counterpart.
  */
 QI4_API int qi4_verify_draft(const int64_t* draft_tokens, const void* target_probs, int64_t target_batch_stride,
                              int64_t target_pos_stride, const void* draft_probs, int64_t draft_batch_stride,

@@ -14,11 +14,12 @@
 // the sums. Where no weight is left (p <= q throughout, after rounding) the
 // token is drawn from p_a; where p_a has none either it is -1.
 //
-// Bound by one pass over two vocabulary rows. One cluster of 16 CTAs per
+// Bound by one pass over two vocabulary rows. One cluster of 8 or 16 CTAs per
 // sequence: each finds `a` for itself (the drafts side by side in one warp),
-// sums its sixteenth of the vocabulary, a contiguous stretch per warp; the
-// sums are exchanged over distributed shared memory, and the one CTA whose
-// stretch holds the drawn share scans it again (from L2) for the token.
+// sums its share of the vocabulary, a contiguous stretch per warp, one sum
+// for every step of the warp's loads; the sums are exchanged over distributed
+// shared memory, and the one warp whose stretch holds the drawn share finds the
+// step among its sums and reads that step again (from L2) for the token.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -33,7 +34,8 @@ __device__ int g_verify_error;
 namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kCluster = 16;
+constexpr int kMaxVocab = 1 << 21;
+constexpr int kMaxSteps = kMaxVocab / (8 * kWarps) / 128;  // steps of a warp at most (of 128 elements at least)
 
 struct VerifyArgs {
   const int64_t* tokens;  // [B, K]
@@ -101,28 +103,58 @@ struct Weights {
   static __device__ __forceinline__ long long units(float w) {
     return __float2ll_rz(fminf(fmaxf(w, 0.f), 1.f) * 1099511627776.f);  // 2^40; a NaN counts as nothing
   }
-  // Elements v .. v + kVec - 1, those from `end` on without weight.
-  __device__ __forceinline__ void load(int v, int end, float (&w)[kVec]) const {
+  // Elements v .. v + kVec - 1 in units, those from `end` on without weight.
+  __device__ __forceinline__ long long load(int v, int end, long long (&n)[kVec]) const {
     float x[kVec], y[kVec];
+    long long sum = 0;
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) x[i] = y[i] = 0.f;
-    if (vec && v + kVec <= end) {
-      Elem<T>::split(__ldg(reinterpret_cast<const uint4*>(p + v)), x);
-      if (q) Elem<T>::split(__ldg(reinterpret_cast<const uint4*>(q + v)), y);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kVec; ++i)
-        if (v + i < end) {
-          x[i] = Elem<T>::get(__ldg(p + v + i));
-          if (q) y[i] = Elem<T>::get(__ldg(q + v + i));
-        }
+    for (int i = 0; i < kVec; ++i) {
+      x[i] = y[i] = 0.f;
+      if (v + i < end) {
+        x[i] = Elem<T>::get(__ldg(p + v + i));
+        if (q) y[i] = Elem<T>::get(__ldg(q + v + i));
+      }
     }
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) w[i] = v + i == skip ? 0.f : x[i] - y[i];
+    for (int i = 0; i < kVec; ++i) sum += n[i] = v + i == skip ? 0 : units(x[i] - y[i]);
+    return sum;
+  }
+  // The sums of kAtOnce whole steps from v on, all their loads at once.
+  template <int kAtOnce>
+  __device__ __forceinline__ void load_whole(int v, long long (&sum)[kAtOnce]) const {
+    uint4 a[kAtOnce], b[kAtOnce];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) a[j] = __ldg(reinterpret_cast<const uint4*>(p + v + j * 32 * kVec));
+    if (q) {
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) b[j] = __ldg(reinterpret_cast<const uint4*>(q + v + j * 32 * kVec));
+    } else {
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) b[j] = make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      float x[kVec], y[kVec];
+      Elem<T>::split(a[j], x);
+      Elem<T>::split(b[j], y);
+      sum[j] = 0;
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) sum[j] += v + j * 32 * kVec + i == skip ? 0 : units(x[i] - y[i]);
+    }
   }
 };
 
-template <int T>
+// Sums over the lanes up to each.
+__device__ __forceinline__ long long scan(long long x, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  return x;
+}
+
+template <int T, int kCluster>
 __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs a) {
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
@@ -131,6 +163,7 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs a) {
   constexpr int kStep = 32 * W::kVec;
   __shared__ int accepted_s, refused_s;
   __shared__ long long warp_sum[kWarps];
+  __shared__ long long step_sum[kWarps][kMaxSteps];
   __shared__ long long cta_sum[2];  // by attempt
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int b = blockIdx.x / kCluster, rank = blockIdx.x % kCluster;
@@ -182,15 +215,34 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs a) {
   long long token = -1;
   for (int attempt = 0; attempt < 2; ++attempt) {
     long long sum = 0;
-#pragma unroll 4
-    for (int v = v0 + lane * W::kVec; v < v1; v += kStep) {
-      float x[W::kVec];
-      w.load(v, v1, x);
+    // A step's sum over the warp: below 32 x kVec x 2^40, so that its halves' sums fit 32 bits.
+    auto keep = [&](long long here, int step) {
+      const long long all = (long long)__reduce_add_sync(0xffffffffu, (unsigned)(here & 0xFFFFFF)) +
+                            ((long long)__reduce_add_sync(0xffffffffu, (unsigned)(here >> 24)) << 24);
+      if (lane == 0) step_sum[warp][step] = all;
+      sum += all;
+    };
+    constexpr int kAtOnce = 4;
+    int step = 0;
+    if (w.vec)
+      for (; v0 + (step + kAtOnce) * kStep <= v1; step += kAtOnce) {
+        long long here[kAtOnce];
+        w.template load_whole<kAtOnce>(v0 + step * kStep + lane * W::kVec, here);
 #pragma unroll
-      for (int i = 0; i < W::kVec; ++i) sum += W::units(x[i]);
+        for (int j = 0; j < kAtOnce; ++j) keep(here[j], step + j);
+      }
+    if (w.vec)
+      for (; v0 + (step + 1) * kStep <= v1; ++step) {
+        long long here[1];
+        w.template load_whole<1>(v0 + step * kStep + lane * W::kVec, here);
+        keep(here[0], step);
+      }
+#pragma unroll 2
+    for (; v0 + step * kStep < v1; ++step) {
+      long long n[W::kVec];
+      keep(w.load(v0 + step * kStep + lane * W::kVec, v1, n), step);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const int steps = step;
     if (lane == 0) warp_sum[warp] = sum;
     __syncthreads();
     if (tid == 0) {
@@ -199,12 +251,8 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs a) {
       cta_sum[attempt] = s;
     }
     cluster.sync();
-    long long theirs = lane < kCluster ? *cluster.map_shared_rank(&cta_sum[attempt], lane) : 0, incl = theirs;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long x = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += x;
-    }
+    const long long theirs = lane < kCluster ? *cluster.map_shared_rank(&cta_sum[attempt], lane) : 0,
+                    incl = scan(theirs, lane);
     const long long total = __shfl_sync(0xffffffffu, incl, 31);
     const long long share = (long long)fminf(fmaxf(__ldg(u + a.K) * 16777216.f, 0.f), 16777215.f);
     const long long goal = share * (total >> 24) + ((share * (total & 0xFFFFFF)) >> 24);
@@ -229,33 +277,29 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs a) {
       }
       if (warp == holder) {
         if (total > 0) {
-          for (int v = v0;; v += kStep) {
-            float x[W::kVec];
-            w.load(v + lane * W::kVec, v1, x);
-            long long n[W::kVec], here = 0;
-#pragma unroll
-            for (int i = 0; i < W::kVec; ++i) here += n[i] = W::units(x[i]);
-            long long run = here;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-              const long long y = __shfl_up_sync(0xffffffffu, run, o);
-              if (lane >= o) run += y;
+          // The step that holds the share, 32 sums at a time, then the element.
+          for (int j0 = 0; j0 < steps && token < 0; j0 += 32) {
+            const long long mine_sum = j0 + lane < steps ? step_sum[warp][j0 + lane] : 0;
+            const long long upto = scan(mine_sum, lane);
+            const unsigned in = __ballot_sync(0xffffffffu, goal < at + upto);
+            if (!in) {
+              at += __shfl_sync(0xffffffffu, upto, 31);
+              continue;
             }
-            const unsigned hit = __ballot_sync(0xffffffffu, at + run > goal);
-            if (hit) {
-              long long s = at + run - here;
-              int k = 0;
+            const int j = __ffs(in) - 1, v = v0 + (j0 + j) * kStep + lane * W::kVec;
+            at += __shfl_sync(0xffffffffu, upto - mine_sum, j);
+            long long n[W::kVec];
+            const long long here = w.load(v, v1, n), run = scan(here, lane);
+            const unsigned hit = __ballot_sync(0xffffffffu, goal < at + run);
+            long long s = at + run - here;
+            int k = 0;
 #pragma unroll
-              for (int i = 0; i < W::kVec - 1; ++i)
-                if (k == i && s + n[i] <= goal) {
-                  s += n[i];
-                  ++k;
-                }
-              token = __shfl_sync(0xffffffffu, v + lane * W::kVec + k, __ffs(hit) - 1);
-              break;
-            }
-            at += __shfl_sync(0xffffffffu, run, 31);
-            if (v >= v1) break;  // (the stretch holds the share, so this is not reached)
+            for (int i = 0; i < W::kVec - 1; ++i)
+              if (k == i && s + n[i] <= goal) {
+                s += n[i];
+                ++k;
+              }
+            token = __shfl_sync(0xffffffffu, v + k, __ffs(hit) - 1);
           }
         }
         int64_t* out = a.out + (int64_t)b * (a.K + 1);
@@ -268,16 +312,19 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs a) {
   cluster.sync();  // no CTA leaves while another may read its sum
 }
 
-template <int T>
-cudaError_t launch_verify(const VerifyArgs& a, int B, cudaStream_t stream) {
-  static std::atomic<unsigned long long> configured{0};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  const unsigned long long bit = 1ull << (dev & 63);
-  if (!(configured.load(std::memory_order_relaxed) & bit)) {
-    const cudaError_t e = cudaFuncSetAttribute(verify_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return e;
-    configured.fetch_or(bit, std::memory_order_relaxed);
+template <int T, int kCluster>
+cudaError_t launch_clusters(const VerifyArgs& a, int B, cudaStream_t stream) {
+  auto kernel = verify_kernel<T, kCluster>;
+  if constexpr (kCluster > 8) {
+    static std::atomic<unsigned long long> configured{0};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (!(configured.load(std::memory_order_relaxed) & bit)) {
+      const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      if (e != cudaSuccess) return e;
+      configured.fetch_or(bit, std::memory_order_relaxed);
+    }
   }
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -291,7 +338,15 @@ cudaError_t launch_verify(const VerifyArgs& a, int B, cudaStream_t stream) {
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, verify_kernel<T>, a);
+  return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
+// Clusters of 16 while the CTAs are at most two per SM (a sequence's time is
+// then the serial path of one: 6.1 us against 7.3 in clusters of 8 for one
+// sequence of 151,936 tokens), else of 8 (64 sequences: 15.9 us against 22.5).
+template <int T>
+cudaError_t launch_verify(const VerifyArgs& a, int B, int sms, cudaStream_t stream) {
+  return (int64_t)B * 16 <= 2 * sms ? launch_clusters<T, 16>(a, B, stream) : launch_clusters<T, 8>(a, B, stream);
 }
 
 }  // namespace
@@ -315,8 +370,8 @@ extern "C" QI4_API int qi4_verify_draft(const int64_t* draft_tokens, const void*
     set_error("draft verification takes FP32, BF16 or FP16 probabilities");
     return QI4_ERR_DTYPE;
   }
-  if (B <= 0 || K < 0 || V <= 0 || B > (1 << 26) || K > 4096 || V > (1 << 22)) {
-    set_error("draft verification: B and V must be positive, K not negative (B <= 2^26, K <= 4096, V <= 2^22; got "
+  if (B <= 0 || K < 0 || V <= 0 || B > (1 << 26) || K > 4096 || V > kMaxVocab) {
+    set_error("draft verification: B and V must be positive, K not negative (B <= 2^26, K <= 4096, V <= 2^21; got "
               "%lld, %lld, %lld)", (long long)B, (long long)K, (long long)V);
     return QI4_ERR_SHAPE;
   }
@@ -330,9 +385,9 @@ extern "C" QI4_API int qi4_verify_draft(const int64_t* draft_tokens, const void*
   VerifyArgs a = {draft_tokens, target_probs, draft_probs, target_batch_stride, target_pos_stride,
                   draft_batch_stride, draft_pos_stride, uniforms, draft_counts, out_tokens, accepted, (int)K, (int)V};
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = dtype == QI4_DTYPE_F32    ? launch_verify<QI4_DTYPE_F32>(a, (int)B, s)
-                        : dtype == QI4_DTYPE_BF16 ? launch_verify<QI4_DTYPE_BF16>(a, (int)B, s)
-                                                  : launch_verify<QI4_DTYPE_F16>(a, (int)B, s);
+  const cudaError_t e = dtype == QI4_DTYPE_F32    ? launch_verify<QI4_DTYPE_F32>(a, (int)B, sms, s)
+                        : dtype == QI4_DTYPE_BF16 ? launch_verify<QI4_DTYPE_BF16>(a, (int)B, sms, s)
+                                                  : launch_verify<QI4_DTYPE_F16>(a, (int)B, sms, s);
   if (e != cudaSuccess) {
     cudaGetLastError();
     set_error("draft verification launch failed: %s", cudaGetErrorString(e));
