@@ -413,72 +413,89 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the pieces of the item that begins in CTA blockIdx.x's run and ends
-// beyond it, if there is one; a block for each row. Groups of D / 4 lanes take
-// the pieces by turns, up to eight at once (one round of loads for 64 or 128
-// pieces), then their sums meet in shared memory in the groups' order.
-constexpr int kJoinThreads = 256;
+// Joins the pieces of the split items. Groups of D / 4 lanes, eight pieces'
+// loads under way in each: of an item of few pieces every group takes a row; of
+// one of many the groups share a row's pieces, and their sums meet in shared
+// memory in the groups' order.
 template <int D, int R, bool F16>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArgs a) {
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArgs a, int ctas) {
   constexpr int kLanes = D / 4, kGroups = kJoinThreads / kLanes, kAtOnce = 8;
   constexpr int64_t kSlot = (int64_t)R * (D + 2);
   __shared__ float4 acc_s[kGroups][kLanes];
   __shared__ float2 ml_s[kGroups];
+  __shared__ int ends[kMaxCtas];
   pdl_launch_dependents();  // (what follows waits for this launch, and it for the one before)
   pdl_wait();
-  const SplitItem it = a.splits[blockIdx.x];
-  const int r = blockIdx.y, np = it.pieces;
-  if (r >= it.rows) return;
+  const int total = count_shares(a.splits, ctas, ends, [](int pieces, int rows) {
+    return pieces <= kAtOnce ? (rows + kGroups - 1) / kGroups : rows;
+  });
   const int group = threadIdx.x / kLanes, d = (threadIdx.x % kLanes) * 4;
-  const float* first = a.ws + it.slot * kSlot;
-  const float* later = a.ws + 2 * (int64_t)blockIdx.x * kSlot;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float top = -INFINITY, l = 0.f;
-  for (int q0 = group; q0 < np; q0 += kGroups * kAtOnce) {
-    float2 ml[kAtOnce];
-    float4 v[kAtOnce];
+  for (int u = blockIdx.x; u < total; u += gridDim.x) {
+    int part;
+    const int c = share_owner(ends, ctas, u, part);
+    const SplitItem it = a.splits[c];
+    const int np = it.pieces;
+    const bool many = np > kAtOnce;
+    const int r = many ? part : part * kGroups + group;
+    const float* first = a.ws + it.slot * kSlot;
+    const float* later = a.ws + 2 * (int64_t)c * kSlot;
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    float top = -INFINITY, l = 0.f;
+    if (r < it.rows) {
+      const int step = many ? kGroups : 1;
+      for (int q0 = many ? group : 0; q0 < np; q0 += step * kAtOnce) {
+        float2 ml[kAtOnce];
+        float4 v[kAtOnce];
 #pragma unroll
-    for (int j = 0; j < kAtOnce; ++j) {
-      const int p = q0 + j * kGroups;
-      ml[j] = make_float2(-INFINITY, 0.f);
-      v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (p < np) {
-        const float* src = p ? later + 2 * p * kSlot : first;
-        ml[j] = *reinterpret_cast<const float2*>(src + R * D + 2 * r);
-        v[j] = *reinterpret_cast<const float4*>(src + r * D + d);
+        for (int j = 0; j < kAtOnce; ++j) {
+          const int p = q0 + j * step;
+          ml[j] = make_float2(-INFINITY, 0.f);
+          v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (p < np) {
+            const float* src = p ? later + 2 * p * kSlot : first;
+            ml[j] = *reinterpret_cast<const float2*>(src + R * D + 2 * r);
+            v[j] = *reinterpret_cast<const float4*>(src + r * D + d);
+          }
+        }
+        float to = top;
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) to = fmaxf(to, ml[j].x);
+        const float base = to == -INFINITY ? 0.f : to, back = exp2_approx(top - base);
+        top = to;
+        l *= back;
+        x[0] *= back, x[1] *= back, x[2] *= back, x[3] *= back;
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) {
+          const float f = exp2_approx(ml[j].x - base);
+          l += ml[j].y * f;
+          x[0] += v[j].x * f, x[1] += v[j].y * f, x[2] += v[j].z * f, x[3] += v[j].w * f;
+        }
       }
     }
-    float to = top;
+    if (many) {  // (the same for every thread of the block)
+      acc_s[group][threadIdx.x % kLanes] = make_float4(x[0], x[1], x[2], x[3]);
+      if (d == 0) ml_s[group] = make_float2(top, l);
+      __syncthreads();
+      if (group == 0) {
+        top = -INFINITY, l = 0.f;
+        x[0] = x[1] = x[2] = x[3] = 0.f;
 #pragma unroll
-    for (int j = 0; j < kAtOnce; ++j) to = fmaxf(to, ml[j].x);
-    const float base = to == -INFINITY ? 0.f : to, back = exp2_approx(top - base);
-    top = to;
-    l *= back;
-    acc = make_float4(acc.x * back, acc.y * back, acc.z * back, acc.w * back);
+        for (int g = 0; g < kGroups; ++g) top = fmaxf(top, ml_s[g].x);
+        const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
-    for (int j = 0; j < kAtOnce; ++j) {
-      const float f = exp2_approx(ml[j].x - base);
-      l += ml[j].y * f;
-      acc = make_float4(acc.x + v[j].x * f, acc.y + v[j].y * f, acc.z + v[j].z * f, acc.w + v[j].w * f);
+        for (int g = 0; g < kGroups; ++g) {
+          const float f = exp2_approx(ml_s[g].x - base);
+          const float4 v = acc_s[g][threadIdx.x];
+          l += ml_s[g].y * f;
+          x[0] += v.x * f, x[1] += v.y * f, x[2] += v.z * f, x[3] += v.w * f;
+        }
+      }
     }
-  }
-  acc_s[group][threadIdx.x % kLanes] = acc;
-  if (d == 0) ml_s[group] = make_float2(top, l);
-  __syncthreads();
-  if (group == 0) {
-    float to = -INFINITY, sum = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g) to = fmaxf(to, ml_s[g].x);
-    const float base = to == -INFINITY ? 0.f : to;
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-      const float f = exp2_approx(ml_s[g].x - base);
-      const float4 v = acc_s[g][threadIdx.x];
-      sum += ml_s[g].y * f;
-      x[0] += v.x * f, x[1] += v.y * f, x[2] += v.z * f, x[3] += v.w * f;
+    if (r < it.rows && (!many || group == 0)) {
+      const int row = it.row0 + r, token = a.by_G(row);
+      finish_row<D, F16, 4>(a, it.first + token, it.kvh * a.G + row - token * a.G, d, x, top, l);
     }
-    const int row = it.row0 + r, token = a.by_G(row);
-    finish_row<D, F16, 4>(a, it.first + token, it.kvh * a.G + row - token * a.G, d, x, to, sum);
+    if (many) __syncthreads();  // the next share's sums replace these
   }
 }
 
@@ -488,12 +505,12 @@ cudaError_t launch_join(const PagedArgs& a, int ctas, cudaStream_t s) {
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)ctas, R, 1);
+  cfg.gridDim = dim3((unsigned)(kJoinBlocksPerSm * ctas), 1, 1);
   cfg.blockDim = dim3(kJoinThreads, 1, 1);
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_join_kernel<D, R, F16>, a);
+  return cudaLaunchKernelEx(&cfg, paged_join_kernel<D, R, F16>, a, ctas);
 }
 
 }  // namespace
@@ -642,6 +659,7 @@ int attend(const Call& c, const char* what) {
   int sms = 0;
   rc = require_device(&sms);
   if (rc) return rc;
+  if (sms > kMaxCtas) sms = kMaxCtas;  // (CTAs of a launch; a B200 has 148)
   const size_t need = workspace_bytes_for(c.T, c.Hq, kv.kv_heads, D, most, prefix, sms);
   char* ws = static_cast<char*>(c.ws);
   if (ws && (c.ws_bytes < need || !al(ws, 16))) {
@@ -751,5 +769,6 @@ extern "C" QI4_API size_t qi4_paged_attention_workspace(int64_t T, int64_t Hq, i
   if (T < 0 || Hq <= 0 || kv_heads <= 0 || Hq % kv_heads || head_dim <= 0 || max_tokens < 0) return 0;
   int sms = 0;
   if (qi4::require_device(&sms)) return 0;
+  sms = std::min(sms, qi4::kMaxCtas);
   return qi4::workspace_bytes_for(T, Hq, kv_heads, head_dim, max_tokens ? std::min(max_tokens, T) : T, prefix != 0, sms);
 }

@@ -21,6 +21,7 @@
 namespace qi4 {
 
 constexpr int kBlockKeys = 128;  // keys of a unit
+constexpr int kMaxCtas = 256;    // CTAs of a launch at most
 
 struct PagedArgs {
   const uint16_t* q;
@@ -54,8 +55,8 @@ struct PagedArgs {
 // An item whose pieces are joined: `pieces` of them (0: none), the first in
 // slot `slot`, piece p > 0 in slot 2 (cta + p). Row r of its tile is query row
 // row0 + r of the sequence whose first token is `first`.
-struct SplitItem {
-  int pieces, slot, rows, first, row0, kvh;
+struct alignas(8) SplitItem {
+  int pieces, rows, slot, first, row0, kvh;
 };
 
 // The dealing of U units to C CTAs: CTA c owns [start(c), start(c + 1)),
@@ -339,8 +340,61 @@ template <int R>
 __device__ __forceinline__ void note_split(const PagedArgs& a, const Walk<R>& w, bool any) {
   SplitItem it = {0, 0, 0, 0, 0, 0};
   if (any && w.blk == 0 && w.nblk > 0 && !w.whole())
-    it = {w.pieces(), w.slot(blockIdx.x), w.rows(a), w.first, w.row0(a), w.kvh};
+    it = {w.pieces(), w.rows(a), w.slot(blockIdx.x), w.first, w.row0(a), w.kvh};
   a.splits[blockIdx.x] = it;
+}
+
+// The joining launches: every block learns of all split items (one entry per
+// CTA of the launch before) and takes every gridDim.x-th of their shares.
+// Blocks that own (CTA, rows) places instead, most of them empty, took two to
+// three times as long: thousands of blocks, each a round trip to memory.
+constexpr int kJoinThreads = 256;
+constexpr int kJoinBlocksPerSm = 4;
+
+// ends[c]: shares of the items noted by CTAs 0 .. c; `shares` of an item as given. All threads of the block take part.
+template <class Shares>
+__device__ __forceinline__ int count_shares(const SplitItem* splits, int ctas, int* ends, const Shares& shares) {
+  __shared__ int warp_sum[kJoinThreads / 32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int before = 0;
+  for (int c0 = 0; c0 < ctas; c0 += kJoinThreads) {
+    const int c = c0 + threadIdx.x;
+    int x = 0;
+    if (c < ctas) {
+      const int2 head = *reinterpret_cast<const int2*>(&splits[c].pieces);
+      x = head.x ? shares(head.x, head.y) : 0;
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) warp_sum[warp] = x;
+    __syncthreads();
+    int all = 0;
+#pragma unroll
+    for (int i = 0; i < kJoinThreads / 32; ++i) {
+      if (i == warp) x += before + all;
+      all += warp_sum[i];
+    }
+    if (c < ctas) ends[c] = x;
+    before += all;
+    __syncthreads();
+  }
+  return before;
+}
+// The CTA whose item has share u, and the share's number within the item.
+__device__ __forceinline__ int share_owner(const int* ends, int ctas, int u, int& within) {
+  int lo = 0, hi = ctas - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (ends[mid] <= u)
+      lo = mid + 1;
+    else
+      hi = mid;
+  }
+  within = u - (lo ? ends[lo - 1] : 0);
+  return lo;
 }
 
 // Launch of the tcgen05 kernel (paged_prefill.cu): tiles of kTcRows rows.

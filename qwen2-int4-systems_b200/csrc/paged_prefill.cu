@@ -32,7 +32,6 @@
 // a product of N = 64 with both operands in shared memory takes the 64 cycles
 // of one with N = 128.)
 // Tensor memory: scores 2 x 128 columns, sums 2 x D. All waits are bounded.
-#include <algorithm>
 #include <atomic>
 
 #include "paged_attention.cuh"
@@ -448,70 +447,99 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the pieces of the item that begins in CTA blockIdx.x's run and ends
-// beyond it, if there is one: block (c, y, z) takes 32 rows and 32 dims. A
-// piece is [D][kTcRows] sums, then [kTcRows] (max, sum): lanes are rows, eight
-// pieces' loads under way at once.
-constexpr int kJoinThreads = 256;
-template <int D, bool F16>
-__global__ void __launch_bounds__(kJoinThreads) paged_tc_join_kernel(const PagedArgs a) {
+// Joins the pieces of the split items. A piece is [D][kTcRows] sums, then
+// [kTcRows] (max, sum): lanes are rows. A share is 32 rows: all dims of an item
+// of few pieces, 32 dims of one of many, each warp an eighth of them, with 32
+// loads under way in every thread.
+template <int D, bool F16, int kPieces, int kDims>
+__device__ __forceinline__ void join_rows(const float* first, const float* later, int np, int d, int r, float (&acc)[kDims],
+                                          float& top, float& l) {
   constexpr int64_t kSlot = (int64_t)kTcRows * (D + 2);
-  constexpr int kAtOnce = 8;
-  __shared__ float out_s[32][33], top_s[32], l_s[32];
-  pdl_launch_dependents();
-  pdl_wait();
-  const SplitItem it = a.splits[blockIdx.x];
-  const int r0 = 32 * blockIdx.y, np = it.pieces;
-  if (r0 >= it.rows) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = r0 + lane;
-  const int d0 = 4 * warp, d = 32 * blockIdx.z + d0;
-  const float* first = a.ws + it.slot * kSlot;
-  const float* later = a.ws + 2 * (int64_t)blockIdx.x * kSlot;
-  float acc[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f, top = -INFINITY;
-  for (int p0 = 0; p0 < np; p0 += kAtOnce) {
-    float v[kAtOnce][4];
-    float2 ml[kAtOnce];
 #pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) {
+  for (int k = 0; k < kDims; ++k) acc[k] = 0.f;
+  top = -INFINITY, l = 0.f;
+  for (int p0 = 0; p0 < np; p0 += kPieces) {
+    float v[kPieces][kDims];
+    float2 ml[kPieces];
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
       const int p = p0 + i;
       ml[i] = make_float2(-INFINITY, 0.f);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[i][k] = 0.f;
+      for (int k = 0; k < kDims; ++k) v[i][k] = 0.f;
       if (p < np) {
         const float* src = p ? later + 2 * p * kSlot : first;
         ml[i] = *reinterpret_cast<const float2*>(src + (int64_t)kTcRows * D + 2 * r);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[i][k] = src[(d + k) * kTcRows + r];
+        for (int k = 0; k < kDims; ++k) v[i][k] = src[(d + k) * kTcRows + r];
       }
     }
     float to = top;
 #pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) to = fmaxf(to, ml[i].x);
+    for (int i = 0; i < kPieces; ++i) to = fmaxf(to, ml[i].x);
     const float base = to == -INFINITY ? 0.f : to, back = exp2_approx(top - base);
     top = to;
     l *= back;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) acc[k] *= back;
+    for (int k = 0; k < kDims; ++k) acc[k] *= back;
 #pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) {
+    for (int i = 0; i < kPieces; ++i) {
       const float f = exp2_approx(ml[i].x - base);
       l += ml[i].y * f;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) acc[k] += v[i][k] * f;
+      for (int k = 0; k < kDims; ++k) acc[k] += v[i][k] * f;
     }
   }
+}
+
+template <int D, bool F16>
+__global__ void __launch_bounds__(kJoinThreads) paged_tc_join_kernel(const PagedArgs a, int ctas) {
+  constexpr int64_t kSlot = (int64_t)kTcRows * (D + 2);
+  constexpr int kFew = 4;
+  __shared__ float out_s[32][D + 1], top_s[32], l_s[32];
+  __shared__ int ends[kMaxCtas];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int total = count_shares(a.splits, ctas, ends, [](int pieces, int rows) {
+    return (rows + 31) / 32 * (pieces <= kFew ? 1 : D / 32);
+  });
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int u = blockIdx.x; u < total; u += gridDim.x) {
+    int part;
+    const int c = share_owner(ends, ctas, u, part);
+    const SplitItem it = a.splits[c];
+    const bool few = it.pieces <= kFew;
+    const int z = few ? 0 : part % (D / 32), r0 = 32 * (few ? part : part / (D / 32));
+    const int r = min(r0 + lane, kTcRows - 1), dims = few ? D : 32;
+    const float* first = a.ws + it.slot * kSlot;
+    const float* later = a.ws + 2 * (int64_t)c * kSlot;
+    float top, l;
+    if (few) {
+      constexpr int kEach = D / 8;
+      float acc[kEach];
+      join_rows<D, F16, 2, kEach>(first, later, it.pieces, kEach * warp, r, acc, top, l);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) out_s[lane][d0 + k] = acc[k];
-  if (warp == 0) top_s[lane] = top, l_s[lane] = l;
-  __syncthreads();
-  const int orow = threadIdx.x / 8, od = (threadIdx.x % 8) * 4;
-  if (r0 + orow < it.rows) {
-    float x[4];
+      for (int k = 0; k < kEach; ++k) out_s[lane][kEach * warp + k] = acc[k];
+    } else {
+      float acc[4];
+      join_rows<D, F16, 8, 4>(first, later, it.pieces, 32 * z + 4 * warp, r, acc, top, l);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) x[k] = out_s[orow][od + k];
-    const int row = it.row0 + r0 + orow, token = a.by_G(row);
-    finish_row<D, F16, 4>(a, it.first + token, it.kvh * a.G + row - token * a.G, 32 * blockIdx.z + od, x, top_s[orow],
-                          l_s[orow]);
+      for (int k = 0; k < 4; ++k) out_s[lane][4 * warp + k] = acc[k];
+    }
+    if (warp == 0) top_s[lane] = top, l_s[lane] = l;
+    __syncthreads();
+    for (int i = threadIdx.x; i < 32 * dims / 4; i += kJoinThreads) {
+      const int orow = i / (dims / 4), od = (i - orow * (dims / 4)) * 4;
+      if (r0 + orow < it.rows) {
+        float x[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = out_s[orow][od + k];
+        const int row = it.row0 + r0 + orow, token = a.by_G(row);
+        finish_row<D, F16, 4>(a, it.first + token, it.kvh * a.G + row - token * a.G, 32 * z + od, x, top_s[orow],
+                              l_s[orow]);
+      }
+    }
+    __syncthreads();  // the next share's sums replace these
   }
 }
 
@@ -540,12 +568,10 @@ cudaError_t launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap
   cfg.numAttrs = 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, q, k, v, a);
   if (e != cudaSuccess) return e;
-  // (No tile has more rows than the whole batch.)
-  const int64_t rows = std::min<int64_t>(a.tile_rows, (int64_t)a.r.T * a.G);
-  cfg.gridDim = dim3((unsigned)ctas, (unsigned)((rows + 31) / 32), D / 32);
+  cfg.gridDim = dim3((unsigned)(kJoinBlocksPerSm * ctas), 1, 1);
   cfg.blockDim = dim3(kJoinThreads, 1, 1);
   cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, paged_tc_join_kernel<D, F16>, a);
+  return cudaLaunchKernelEx(&cfg, paged_tc_join_kernel<D, F16>, a, ctas);
 }
 
 }  // namespace
