@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(kThreads) gemv_argmax_kernel(const __nv_bfloat
     }
   }
   __syncthreads();
-  if (tid < M) {
+  if (keys && tid < M) {  // (null: only the logits are wanted)
     float bv = -INFINITY;
     long long br = -1;
     for (int w = 0; w < kThreads / 32; ++w) {
