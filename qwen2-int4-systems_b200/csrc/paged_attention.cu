@@ -543,7 +543,7 @@ cudaError_t launch_decode(const CUtensorMap& k, const CUtensorMap& v, const Page
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, k, v, a);
-  return e != cudaSuccess ? e : launch_join<D, 8 * NT, F16>(a, ctas, s);
+  return e != cudaSuccess || a.unsplit ? e : launch_join<D, 8 * NT, F16>(a, ctas, s);
 }
 
 template <int D, bool F16>
@@ -566,6 +566,19 @@ cudaError_t launch_kernel(int D, bool f16, int nt, const CUtensorMap& k, const C
 // negative).
 constexpr int64_t kTcFrom = 33;
 bool takes_tc(int64_t tokens, int64_t G, float scale) { return tokens * G >= kTcFrom && G <= 128 && scale >= 0.f; }
+
+// Where the tables cover at most this many keys, an item is one CTA's work and
+// no joining launch follows; half as many for mma.sync items that are fewer
+// than half the CTAs. Lengths are on the device: the tables' width is what the
+// host knows. Split and whole, us: 64 sequences of 500 keys, 12 query heads on
+// 2 KV heads of 128 dims 15.3 and 12.0; 1 sequence of 250 keys 8.5 and 7.1, of
+// 500 8.4 and 9.9; 16 prompts of 500 tokens 42.5 and 37.1, 1 prompt of 200 16.4
+// and 13.3, of 500 18.1 and 17.6. More keys are split although even batches
+// would still gain (64 sequences of 1000 keys: 20.7 and 18.0), for the sake of
+// batches with one long sequence among short ones (alone at 1000 keys: 8.6 and
+// 15.8). A shared prefix, few long items of one length, is always split (500
+// keys under 64 sequences: 23.1 and 27.6).
+constexpr int kWholeKeys = 512;
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 // Room for the pieces of a launch over `tokens` per sequence, and what the runs note of their split items.
@@ -705,6 +718,7 @@ int attend(const Call& c, const char* what) {
     x.by_tile_rows = FastDiv::of(x.tile_rows);
     x.by_G = FastDiv::of(G);
     x.by_ctas = FastDiv::of(sms);
+    x.unsplit = !x.late && x.cap <= (tc || (int64_t)x.r.B * x.Hkv * 2 >= sms ? kWholeKeys : kWholeKeys / 2);
     x.splits = reinterpret_cast<SplitItem*>(at + (size_t)sms * 2 * rows * (D + 2) * sizeof(float));
     if (tc) return launch_paged_tc(D, f16, qmap, kmap, vmap, x, sms, c.stream);
     return launch_kernel(D, f16, R / 8, kmap, vmap, x, sms, c.stream);

@@ -34,6 +34,7 @@ struct PagedArgs {
   int fixed_len;  // >= 0: every sequence has this many keys (lengths is not read)
   int Hkv, G, cap;
   int causal;
+  int unsplit;                 // an item is all done by the CTA that owns its first unit: nothing is joined
   int one_tile;                // no sequence has more rows than a tile (decode steps, drafts): the split is shorter
   int tile_rows, tile_tokens;  // R rows, or the most whole tokens that R rows hold (0 tokens: a token has more rows)
   FastDiv by_tile_rows, by_G, by_ctas;  // by_ctas: the launch's CTAs
@@ -249,7 +250,14 @@ struct Walk {
           blocks = blocks_of(a, tile);
         }
       }
-      const int take = min(1 + blocks - at, end - u);
+      int take = 1 + blocks - at;
+      if (!a.unsplit) {
+        take = min(take, end - u);
+      } else if (at > 0) {  // the item belongs to an earlier CTA
+        u += take;
+        at += take;
+        continue;
+      }
       item0 = u - at;
       blk = max(at - 1, 0);
       nblk = at + take - 1 - blk;

@@ -111,16 +111,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-      : "memory");
-}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Descriptor of V as the second product's B operand: rows are keys (the
@@ -451,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // [kTcRows] (max, sum): lanes are rows. A share is 32 rows: all dims of an item
 // of few pieces, 32 dims of one of many, each warp an eighth of them, with 32
 // loads under way in every thread.
-template <int D, bool F16, int kPieces, int kDims>
+template <int D, int kPieces, int kDims>
 __device__ __forceinline__ void join_rows(const float* first, const float* later, int np, int d, int r, float (&acc)[kDims],
                                           float& top, float& l) {
   constexpr int64_t kSlot = (int64_t)kTcRows * (D + 2);
@@ -517,12 +507,12 @@ __global__ void __launch_bounds__(kJoinThreads) paged_tc_join_kernel(const Paged
     if (few) {
       constexpr int kEach = D / 8;
       float acc[kEach];
-      join_rows<D, F16, 2, kEach>(first, later, it.pieces, kEach * warp, r, acc, top, l);
+      join_rows<D, 2, kEach>(first, later, it.pieces, kEach * warp, r, acc, top, l);
 #pragma unroll
       for (int k = 0; k < kEach; ++k) out_s[lane][kEach * warp + k] = acc[k];
     } else {
       float acc[4];
-      join_rows<D, F16, 8, 4>(first, later, it.pieces, 32 * z + 4 * warp, r, acc, top, l);
+      join_rows<D, 8, 4>(first, later, it.pieces, 32 * z + 4 * warp, r, acc, top, l);
 #pragma unroll
       for (int k = 0; k < 4; ++k) out_s[lane][4 * warp + k] = acc[k];
     }
@@ -567,7 +557,7 @@ cudaError_t launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, q, k, v, a);
-  if (e != cudaSuccess) return e;
+  if (e != cudaSuccess || a.unsplit) return e;
   cfg.gridDim = dim3((unsigned)(kJoinBlocksPerSm * ctas), 1, 1);
   cfg.blockDim = dim3(kJoinThreads, 1, 1);
   cfg.dynamicSmemBytes = 0;

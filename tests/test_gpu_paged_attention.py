@@ -223,3 +223,36 @@ def test_attention_refuses(b200, cuda_device):
                                  (5, pre[None], ValueError)):
         with pytest.raises(error):
             b200.b200_shared_prefix_attention(x["q"], x["k"], x["v"], table, length, x["table"], x["lengths"])
+
+
+MANY = [(1, 1 + 7 * i) for i in range(70)]
+
+
+@pytest.mark.parametrize("prefix", [0, 300])
+@pytest.mark.parametrize("seqs,Hq,Hkv,D,dtype", [
+    (MANY, 12, 2, 128, BF16),                                                    # one row tile each, many of them
+    ([(n % 6, 500 - 9 * n) for n in range(40)], 16, 4, 64, F16),                 # some without tokens
+    ([(3, 255)], 12, 2, 128, BF16),                                              # few
+    ([(1, 0), (4, 2), (2, 250)], 8, 8, 64, BF16),                                # rows that see nothing
+    ([(300, 512), (0, 40), (1, 77), (130, 130), (60, 0)], 12, 2, 128, F16),      # several row tiles
+    ([(40 + i, 40 + 11 * i) for i in range(37)], 4, 1, 64, BF16),
+])
+def test_short_tables_and_wide_ones(b200, cuda_device, seqs, Hq, Hkv, D, dtype, prefix):
+    """The width of the table decides whether the work on a sequence is split: both ways give the attention."""
+    x = pg.build(seqs, Hq=Hq, Hkv=Hkv, D=D, page=8, dtype=dtype, device=cuda_device, prefix=prefix, wide=0)
+    assert x["table"].shape[1] * 8 <= 512
+    wide = torch.full((len(seqs), 400), -1, dtype=torch.int32, device=cuda_device)
+    wide[:, :x["table"].shape[1]] = x["table"]
+    for table in (x["table"], wide):
+        y = dict(x, table=table)
+
+        def run():
+            if not prefix:
+                return _run(b200, y, max_tokens=y["most"])
+            return b200.b200_shared_prefix_attention(y["q"], y["k"], y["v"], y["prefix_table"], prefix, table,
+                                                     y["lengths"], cu_tokens=y["cu"], max_tokens=y["most"])
+
+        out = run()
+        pg.check_attention(out, y)
+        assert torch.equal(out, run())
+    assert _status(b200) == 0
