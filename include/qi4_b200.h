@@ -450,13 +450,13 @@ QI4_API int qi4_rope_paged_append(const qi4_paged_kv* kv, const void* q, int64_t
  * 16 bits or more where a tile has few rows, and rounded to the cache's type
  * on the tcgen05 path (max_tokens * Hq / kv_heads large). What page slots
  * beyond a length hold does not matter, NaN included. q as in
- * qi4_rope_paged_append; out [T, Hq, head_dim] contiguous, 32-byte aligned;
- * head_dim 64 or 128.
+ * qi4_rope_paged_append, its strides positive; out [T, Hq, head_dim]
+ * contiguous, 32-byte aligned; head_dim 64 or 128.
  * max_tokens: no sequence has more new tokens (0: not known); it chooses the
- * kernel and its tiles. workspace: qi4_paged_attention_workspace bytes, 16-byte aligned,
- * no initialisation needed, not shared by calls that may overlap; NULL: the
- * library's scratch pool. Replaces, for a paged cache, reference
- * src/qwen_int4/model.py:90-118.
+ * kernel and its tiles. workspace: qi4_paged_attention_workspace bytes,
+ * 16-byte aligned, no initialisation needed, not shared by calls that may
+ * overlap; NULL: the library's scratch pool. Replaces, for a paged cache,
+ * reference src/qwen_int4/model.py:90-118.
  */
 QI4_API int qi4_paged_attention(const qi4_paged_kv* kv, const void* q, int64_t q_token_stride,
                                 int64_t q_head_stride, void* out, int64_t T, int64_t B, int64_t Hq,

@@ -639,8 +639,9 @@ int attend(const Call& c, const char* what) {
     return QI4_ERR_SHAPE;
   }
   auto al = [](const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
-  if (!al(c.q, 16) || !al(c.out, 32) || c.q_tok % 8 || c.q_head % 8 || c.q_tok < 0 || c.q_head < 0) {
-    set_error("%s: q must be 16-byte and out 32-byte aligned, q with strides that are multiples of 8 elements", what);
+  if (!al(c.q, 16) || !al(c.out, 32) || c.q_tok % 8 || c.q_head % 8 || c.q_tok < (c.T > 1) || c.q_head < (c.Hq > 1)) {
+    set_error("%s: q must be 16-byte and out 32-byte aligned, q with positive strides that are multiples of 8 elements",
+              what);
     return QI4_ERR_ALIGNMENT;
   }
   const bool prefix = c.prefix_len > 0;

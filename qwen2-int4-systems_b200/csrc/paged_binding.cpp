@@ -48,11 +48,11 @@ void want_type(bool ok, const char* message) {
 bool aligned16(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
 
 // [T, heads, D] as the kernels read it: D contiguous, the start 16-byte
-// aligned, strides in whole 16 bytes; copied otherwise.
+// aligned, strides in whole 16 bytes and not zero (an expanded tensor); copied
+// otherwise.
 at::Tensor rows(const at::Tensor& t) {
-  if (t.stride(2) == 1 && aligned16(t) && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && t.stride(0) >= 0 &&
-      t.stride(1) >= 0)
-    return t;
+  auto fits = [&](int64_t dim) { return t.stride(dim) % 8 == 0 && (t.stride(dim) > 0 || t.size(dim) == 1); };
+  if (t.stride(2) == 1 && aligned16(t) && fits(0) && fits(1)) return t;
   const at::Tensor c = t.contiguous();
   return aligned16(c) ? c : c.clone();
 }

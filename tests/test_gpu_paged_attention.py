@@ -256,3 +256,17 @@ def test_short_tables_and_wide_ones(b200, cuda_device, seqs, Hq, Hkv, D, dtype, 
         pg.check_attention(out, y)
         assert torch.equal(out, run())
     assert _status(b200) == 0
+
+
+@pytest.mark.parametrize("tokens", [1, 3, 90])
+def test_queries_in_other_orders(b200, cuda_device, tokens):
+    """Heads major in memory, one row expanded to all tokens, one head expanded to all heads."""
+    x = pg.build([(tokens, tokens + 200), (tokens, tokens + 31)], Hq=8, Hkv=2, D=128, page=16, dtype=BF16,
+                 device=cuda_device)
+    T, H, D = x["q"].shape
+    major = torch.empty(H, T, D, dtype=BF16, device=cuda_device).transpose(0, 1)
+    major.copy_(x["q"])
+    for q in (major, x["q"][:1].expand(T, H, D), x["q"][:, 1:2].expand(T, H, D), x["q"][:1, :1].expand(T, H, D)):
+        out = b200.b200_paged_attention(q, x["k"], x["v"], x["table"], x["lengths"], cu_tokens=x["cu"])
+        assert torch.equal(out, _run(b200, dict(x, q=q.contiguous())))
+    pg.check_attention(out, dict(x, q=q))

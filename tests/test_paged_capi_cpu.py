@@ -102,3 +102,11 @@ def test_operators_need_a_gpu(b200):
         pytest.skip("a GPU is present")
     with pytest.raises(RuntimeError, match="CUDA device"):
         b200.b200_verify_draft(torch.zeros(1, 1, dtype=torch.int64), torch.ones(1, 2, 4), torch.zeros(1, 2))
+
+
+@pytest.mark.parametrize("token_stride,head_stride", [(0, 128), (1536, 0), (-1536, 128), (1540, 128)])
+def test_attention_refuses_strides_it_cannot_read(b200, token_stride, head_stride):
+    mod = _mod(b200)
+    kv = _kv(mod)
+    assert mod.load().qi4_paged_attention(ctypes.byref(kv), FAKE, token_stride, head_stride, FAKE, 4, 4, 12, None, FAKE,
+                                          0, 0.1, 1, None, 0, None) == -4
