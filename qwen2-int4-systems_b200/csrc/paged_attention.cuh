@@ -5,14 +5,14 @@
 // of one KV head - and every item into units of kBlockKeys keys that its rows
 // see. The units of all items, in one line, are dealt to the CTAs in equal
 // runs, so sequences of any mixture of lengths keep all SMs equally busy; a
-// CTA's run may end inside an item. An item wholly inside one run is finished there; the pieces of
-// another go to a workspace as (weighted sums, max, sum of weights), and a
-// second, small launch joins them in the order of the runs, so no result
-// depends on timing. (It is resident before the first launch ends, by
-// programmatic dependent launch. Counting the pieces in the kernel instead,
-// the last CTA of an item joining them, cost 25 us where 74 CTAs met at one
-// counter and one of them read all their pieces: 65 us for one sequence of
-// 131,002 keys against 32 with the second launch.)
+// CTA's run may end inside an item. An item wholly inside one run is finished
+// there; the pieces of another go to a workspace as (weighted sums, max, sum of
+// weights), and a second, small launch joins them in the order of the runs, so
+// no result depends on timing. (Counting the pieces in the kernel instead, the
+// last CTA of an item joining them, cost 25 us where 74 CTAs met at one counter
+// and one of them read all their pieces: 65 us for one sequence of 131,002 keys
+// against 32 then with the second launch.) The second launch is 3 us of a small
+// call, so where tables are short no item is split (`unsplit`).
 #pragma once
 
 #include "paged.cuh"
@@ -355,7 +355,8 @@ __device__ __forceinline__ void note_split(const PagedArgs& a, const Walk<R>& w,
 // The joining launches: every block learns of all split items (one entry per
 // CTA of the launch before) and takes every gridDim.x-th of their shares.
 // Blocks that own (CTA, rows) places instead, most of them empty, took two to
-// three times as long: thousands of blocks, each a round trip to memory.
+// three times as long: thousands of blocks, each a round trip to memory. (Two
+// blocks per SM in place of four were slower, eight gained 1 us of 230 at most.)
 constexpr int kJoinThreads = 256;
 constexpr int kJoinBlocksPerSm = 4;
 

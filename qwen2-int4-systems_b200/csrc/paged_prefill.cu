@@ -32,6 +32,18 @@
 // a product of N = 64 with both operands in shared memory takes the 64 cycles
 // of one with N = 128.)
 // Tensor memory: scores 2 x 128 columns, sums 2 x D. All waits are bounded.
+//
+// Measured (device time, BF16, 12 query heads on 2 KV heads of 128 dims): a
+// prompt of 8192 tokens 230 us, 900 TFLOP/s; six ragged chunks of up to 2047
+// tokens 111 us. A unit takes some 4000 cycles: the tensor cores are active for
+// 46% of them and the exponentials' pipe as long. Neither alone is the bound
+// (230 us become 198 without the exponentials, 213 with an eighth of the
+// products): it is the chain scores - maximum - weights - product of either
+// tile, whose turns interlock only in part. Slower were: the maximum and the
+// weights of a whole unit at once (288 us; 276 with registers moved from the
+// other warps), 16 softmax warps of half a row each (313), a warp for the
+// products of either tile (248), products issued by the softmax warps (266 to
+// 248 then), weights under the old maximum beside the search for the new (241).
 #include <atomic>
 
 #include "paged_attention.cuh"

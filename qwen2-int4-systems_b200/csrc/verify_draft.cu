@@ -20,6 +20,8 @@
 // for every step of the warp's loads; the sums are exchanged over distributed
 // shared memory, and the one warp whose stretch holds the drawn share finds the
 // step among its sums and reads that step again (from L2) for the token.
+// Measured (device time, 151,936 tokens, FP32): one sequence of 4 drafts 6.1 us,
+// all of it latency; 64 of up to 5 drafts 16.0 us, 8.1 of them the rows' bytes.
 #include <cooperative_groups.h>
 
 #include <algorithm>
