@@ -453,7 +453,7 @@ QI4_API int qi4_rope_paged_append(const qi4_paged_kv* kv, const void* q, int64_t
  * qi4_rope_paged_append, its strides positive; out [T, Hq, head_dim]
  * contiguous, 32-byte aligned; head_dim 64 or 128.
  * max_tokens: no sequence has more new tokens (0: not known); it chooses the
- * kernel and its tiles. workspace: qi4_paged_attention_workspace bytes,
+ * kernel and its tiles, and with the width of the block tables the work split. workspace: qi4_paged_attention_workspace bytes,
  * 16-byte aligned, no initialisation needed, not shared by calls that may
  * overlap; NULL: the library's scratch pool. Replaces, for a paged cache,
  * reference src/qwen_int4/model.py:90-118.

@@ -23,12 +23,18 @@
 // further unit 6 to 7 TB/s, so what bounds them is the 9 to 11 us of a call
 // that do not grow with the keys: the launch, each warp's way to its first unit
 // (boundaries, lengths and page table, one after the other), the warps' sums,
-// the joining launch. Sixteen consumer warps in two groups that take the units
+// the joining launch. Few items of tables that cover up to 4096 keys are a
+// cluster's work each, without a joining launch: one sequence of 641 keys 6.3 us.
+// Sixteen consumer warps in two groups that take the units
 // by turns had 96 registers each and were slower (25.1 us for the 64).
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <atomic>
 
 #include "paged_attention.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace qi4 {
 
@@ -40,9 +46,10 @@ constexpr int kWarps = 8;                        // consumer warps
 constexpr int kThreads = 32 * (kWarps + 1);      // and the producer
 constexpr int stages_of(int D) { return D == 128 ? 3 : 6; }
 constexpr int stage_bytes(int D) { return 2 * kBlockKeys * D * 2; }
-constexpr size_t smem_of(int D, int NT) {
+constexpr size_t smem_of(int D, int NT, bool clusters) {
   return 1024 + (size_t)stages_of(D) * stage_bytes(D) + (size_t)8 * NT * (2 * D + 16) +
-         2 * 2 * kWarps * 8 * NT * sizeof(float) + 2 * stages_of(D) * sizeof(uint64_t);
+         2 * 2 * kWarps * 8 * NT * sizeof(float) + 2 * stages_of(D) * sizeof(uint64_t) +
+         (clusters ? 8 * NT * (D + 2) * sizeof(float) : 0);
 }
 
 template <bool F16>
@@ -80,7 +87,10 @@ __device__ __forceinline__ float2 unpack2(uint32_t w) {
   if constexpr (F16) return __half22float2(*reinterpret_cast<const __half2*>(&w));
   return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
 }
-template <int D, int NT, bool F16>
+// kClusters: an item is the work of one cluster, whose CTAs share its units out
+// in order and exchange their sums over distributed shared memory; else the
+// units are dealt to all CTAs (paged_attention.cuh).
+template <int D, int NT, bool F16, bool kClusters>
 __global__ void __launch_bounds__(kThreads, 1)
     paged_decode_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                         const PagedArgs a) {
@@ -94,6 +104,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   float* red_l = red_m + 2 * kWarps * R;
   uint64_t* full = reinterpret_cast<uint64_t*>(red_l + 2 * kWarps * R);
   uint64_t* empty = full + kStages;
+  float* part = reinterpret_cast<float*>(empty + kStages);  // kClusters: [R][D] sums, [R] (max, sum)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -112,7 +123,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_launch_dependents();
 
   Walk<R> w;
-  if (!w.begin(a, lane)) {
+  if constexpr (kClusters) {
+    const int C = (int)cg::this_cluster().num_blocks(), item = (int)blockIdx.x / C;
+    if (!w.share(a, item, (int)blockIdx.x - item * C, C)) return;  // (no tokens: the whole cluster)
+  } else if (!w.begin(a, lane)) {
     if (threadIdx.x == 0) note_split(a, w, false);
     return;
   }
@@ -122,7 +136,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kWarps) {
     // ---- producer: pages -> ring ----
     const int box_rows = 1 << a.box_shift;
-    while (w.next(a)) {
+    for (bool one = true; kClusters ? one : w.next(a); one = false) {
       const int vis = w.tile_visible(a);
       const int nload = w.loaded(vis);
       if (lane == 0 && a.fixed_len < 0 && __ldg(a.r.lengths + w.b) > a.cap) atomicOr(&g_paged_error, kErrCacheFull);
@@ -159,8 +173,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
-    if (lane == 0) note_split(a, w, true);
-    return;
+    if constexpr (!kClusters) {
+      if (lane == 0) note_split(a, w, true);
+      return;
+    }
   }
 
   // ---- consumers ----
@@ -168,9 +184,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int r0 = warp * 16;  // this warp's keys of every unit
   const int lrow = r0 + (lane & 7) + (((lane >> 3) & 1) << 3), lchunk = lane >> 4, lx = lane & 7;
   int par = 0;
-  while (w.next(a)) {
+  for (bool one = warp < kWarps; kClusters ? one : w.next(a); one = false) {
     const int rows = w.rows(a), vis = w.tile_visible(a), nload = w.loaded(vis);
-    if (nload == 0) {  // no row sees a key
+    if (kClusters && nload == 0) {
+      if (threadIdx.x < R) *reinterpret_cast<float2*>(part + R * D + 2 * threadIdx.x) = make_float2(-INFINITY, 0.f);
+    } else if (nload == 0) {  // no row sees a key
       if (a.late) pdl_wait();
       for (int i = threadIdx.x; i < rows * (D / 4); i += 32 * kWarps) {
         const int r = i / (D / 4);
@@ -388,9 +406,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         named_barrier(1, 32 * kWarps);
       }
       constexpr int kLanes = D / 4;
-      if (a.late) pdl_wait();
-      const bool whole = w.whole();
-      float* slot = whole ? nullptr : a.ws + (int64_t)w.slot(blockIdx.x) * (R * (D + 2));
+      if (!kClusters && a.late) pdl_wait();
+      const bool whole = !kClusters && w.whole();
+      float* slot = kClusters ? part : whole ? nullptr : a.ws + (int64_t)w.slot(blockIdx.x) * (R * (D + 2));
       for (int i = threadIdx.x; i < rows * kLanes; i += 32 * kWarps) {
         const int r = i / kLanes, d = (i - r * kLanes) * 4;
         float top = -INFINITY, sum = 0.f;
@@ -419,6 +437,48 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) mbar_arrive(&empty[held]);
       par ^= 1;
     }
+  }
+  if constexpr (kClusters) {
+    // The cluster's CTAs share out the rows' dims; the pieces are joined in their order.
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    if (a.late) pdl_wait();
+    const int C = (int)cluster.num_blocks(), rows = w.rows(a);
+    constexpr int kLanes = D / 4;
+    for (int i = (int)cluster.block_rank() * kThreads + threadIdx.x; i < rows * kLanes; i += C * kThreads) {
+      const int r = i / kLanes, d = (i - r * kLanes) * 4;
+      float acc[4] = {0.f, 0.f, 0.f, 0.f}, top = -INFINITY, sum = 0.f;
+      for (int p0 = 0; p0 < C; p0 += 8) {  // (clusters are of 8 or 16)
+        float2 ml[8];
+        float4 v[8];
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+          const float* there = cluster.map_shared_rank(part, p0 + p);
+          ml[p] = *reinterpret_cast<const float2*>(there + R * D + 2 * r);
+          v[p] = *reinterpret_cast<const float4*>(there + r * D + d);
+        }
+        float to = top;
+#pragma unroll
+        for (int p = 0; p < 8; ++p) to = fmaxf(to, ml[p].x);
+        if (to == -INFINITY) continue;
+        const float back = exp2_approx(top - to);
+        top = to;
+        sum *= back;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[k] *= back;
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+          if (ml[p].x == -INFINITY) continue;  // (its sums may not have been written)
+          const float f = exp2_approx(ml[p].x - to);
+          sum += ml[p].y * f;
+          acc[0] += v[p].x * f, acc[1] += v[p].y * f, acc[2] += v[p].z * f, acc[3] += v[p].w * f;
+        }
+      }
+      int token, head;
+      w.place(a, r, token, head);
+      finish_row<D, F16, 4>(a, token, head, d, acc, top, sum);
+    }
+    cluster.sync();  // no CTA leaves while its sums are read
   }
 }
 
@@ -528,30 +588,74 @@ int read_paged_error(cudaStream_t stream) { return read_error_word(&g_paged_erro
 
 namespace {
 
+// Keys that a table may cover for few items (at most as many as clusters of
+// their CTAs are resident at once) to be the work of a cluster each: one
+// launch, no pieces in memory. Dealt to all SMs and in clusters, us (12 query
+// heads on 2 KV heads of 128 dims): one sequence of 641 keys 8.4 and 6.3, of
+// 4000 8.9 and 8.0; four of 1000 9.0 and 6.3, of 4000 10.6 and 10.4; beyond, the
+// cluster's SMs would be the bound. Clusters of 16 CTAs where the tables cover
+// more than 8 units and so many are resident (2000 keys: one sequence 6.7, four
+// in clusters of 8 7.5), else of 8 (one sequence of 1000 keys 6.1, of 16 6.6).
+constexpr int kClusterKeys = 4096;
+
+template <int D, int NT, bool F16, bool kClusters>
+cudaError_t configure(int dev) {
+  static std::atomic<unsigned long long> configured{0};
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (configured.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  auto kernel = paged_decode_kernel<D, NT, F16, kClusters>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       (int)smem_of(D, NT, kClusters));
+  if (e == cudaSuccess && kClusters) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess) configured.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
+
 template <int D, int NT, bool F16>
 cudaError_t launch_decode(const CUtensorMap& k, const CUtensorMap& v, const PagedArgs& a, int ctas, cudaStream_t s) {
-  auto kernel = paged_decode_kernel<D, NT, F16>;
-  static std::atomic<unsigned long long> configured{0};
   int dev = 0;
   cudaGetDevice(&dev);
-  const unsigned long long bit = 1ull << (dev & 63);
-  if (!(configured.load(std::memory_order_relaxed) & bit)) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_of(D, NT));
-    if (e != cudaSuccess) return e;
-    configured.fetch_or(bit, std::memory_order_relaxed);
-  }
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)ctas, 1, 1);
   cfg.blockDim = dim3(kThreads, 1, 1);
-  cfg.dynamicSmemBytes = smem_of(D, NT);
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, k, v, a);
+  const int64_t items = (int64_t)a.r.B * a.Hkv;
+  if (a.one_tile && !a.unsplit && a.cap <= kClusterKeys && items * 8 <= ctas) {
+    // Clusters that are all resident at once: of 8 CTAs, or of 16 where the tables cover more units than 8.
+    auto kernel = paged_decode_kernel<D, NT, F16, true>;
+    cudaError_t e = configure<D, NT, F16, true>(dev);
+    if (e != cudaSuccess) return e;
+    static std::atomic<int> resident[2][64];  // clusters of 16 and of 8 on a device, plus one
+    cfg.dynamicSmemBytes = smem_of(D, NT, true);
+    cfg.numAttrs = 2;
+    for (int i = a.cap > 8 * kBlockKeys ? 0 : 1; i < 2; ++i) {
+      const int C = 16 >> i;
+      attr[1].val.clusterDim.x = (unsigned)C;
+      cfg.gridDim = dim3((unsigned)(items * C), 1, 1);
+      int fit = resident[i][dev & 63].load(std::memory_order_relaxed) - 1;
+      if (fit < 0) {
+        e = cudaOccupancyMaxActiveClusters(&fit, kernel, &cfg);
+        if (e != cudaSuccess) {
+          cudaGetLastError();
+          fit = 0;
+        }
+        resident[i][dev & 63].store(fit + 1, std::memory_order_relaxed);
+      }
+      if (items <= fit) return cudaLaunchKernelEx(&cfg, kernel, k, v, a);
+    }
+    cfg.numAttrs = 1;
+  }
+  cudaError_t e = configure<D, NT, F16, false>(dev);
+  if (e != cudaSuccess) return e;
+  cfg.gridDim = dim3((unsigned)ctas, 1, 1);
+  cfg.dynamicSmemBytes = smem_of(D, NT, false);
+  e = cudaLaunchKernelEx(&cfg, paged_decode_kernel<D, NT, F16, false>, k, v, a);
   return e != cudaSuccess || a.unsplit ? e : launch_join<D, 8 * NT, F16>(a, ctas, s);
 }
 

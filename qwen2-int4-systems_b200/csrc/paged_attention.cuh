@@ -12,7 +12,9 @@
 // last CTA of an item joining them, cost 25 us where 74 CTAs met at one counter
 // and one of them read all their pieces: 65 us for one sequence of 131,002 keys
 // against 32 then with the second launch.) The second launch is 3 us of a small
-// call, so where tables are short no item is split (`unsplit`).
+// call, so where tables are short no item is split (`unsplit`), and few items of
+// the mma.sync kernel are shared out within clusters (`share`) if their tables
+// are not long.
 #pragma once
 
 #include "paged.cuh"
@@ -224,6 +226,18 @@ struct Walk {
     at -= kvh * (1 + blocks);
     return true;
   }
+  // Instead of a run: part `rank` of `parts` of item `item`, which is a sequence and KV head (one_tile). False if the
+  // sequence has no tokens.
+  __device__ __forceinline__ bool share(const PagedArgs& a, int item, int rank, int parts) {
+    const int seq = item / a.Hkv;
+    load(a, seq);
+    kvh = item - seq * a.Hkv;
+    tile = 0;
+    blocks = blocks_of(a, 0);
+    blk = blocks * rank / parts;
+    nblk = blocks * (rank + 1) / parts - blk;
+    return tiles > 0;
+  }
   // This CTA's run of U units.
   __device__ __forceinline__ bool deal(const PagedArgs& a, int U) {
     if ((int)blockIdx.x >= min((int)gridDim.x, U)) return false;
@@ -346,6 +360,7 @@ __device__ __forceinline__ void finish_row(const PagedArgs& a, int64_t token, in
 // What a CTA leaves for the joining launch, from its last piece (one thread).
 template <int R>
 __device__ __forceinline__ void note_split(const PagedArgs& a, const Walk<R>& w, bool any) {
+  if (a.unsplit) return;
   SplitItem it = {0, 0, 0, 0, 0, 0};
   if (any && w.blk == 0 && w.nblk > 0 && !w.whole())
     it = {w.pieces(), w.rows(a), w.slot(blockIdx.x), w.first, w.row0(a), w.kvh};

@@ -270,3 +270,32 @@ def test_queries_in_other_orders(b200, cuda_device, tokens):
         out = b200.b200_paged_attention(q, x["k"], x["v"], x["table"], x["lengths"], cu_tokens=x["cu"])
         assert torch.equal(out, _run(b200, dict(x, q=q.contiguous())))
     pg.check_attention(out, dict(x, q=q))
+
+
+@pytest.mark.parametrize("prefix", [0, 700])
+@pytest.mark.parametrize("seqs,Hq,Hkv,D,dtype", [
+    ([(1, 641)], 12, 2, 128, BF16),
+    ([(1, 1), (1, 0), (1, 3900), (0, 9), (1, 128)], 12, 2, 128, F16),  # one key, none, no tokens
+    ([(5, 2000), (4, 2), (3, 129), (5, 4000)], 16, 4, 64, F16),       # rows that see nothing; 20 rows
+    ([(4, 3000), (1, 257)], 8, 1, 128, BF16),                         # 32 rows
+    ([(2, 1025)], 8, 8, 64, BF16),
+    ([(1, 300 + 7 * i) for i in range(9)], 16, 2, 128, BF16),         # 18 items
+])
+def test_few_sequences_however_wide_the_table(b200, cuda_device, seqs, Hq, Hkv, D, dtype, prefix):
+    """Tables that cover 4096 keys and more of them: an item as one cluster's work, and dealt to all SMs."""
+    x = pg.build(seqs, Hq=Hq, Hkv=Hkv, D=D, page=16, dtype=dtype, device=cuda_device, prefix=prefix, wide=0)
+    for pages in (x["table"].shape[1], 256, 257):
+        table = torch.full((len(seqs), pages), -1, dtype=torch.int32, device=cuda_device)
+        table[:, :x["table"].shape[1]] = x["table"]
+        y = dict(x, table=table)
+
+        def run():
+            if not prefix:
+                return _run(b200, y, max_tokens=y["most"])
+            return b200.b200_shared_prefix_attention(y["q"], y["k"], y["v"], y["prefix_table"], prefix, table,
+                                                     y["lengths"], cu_tokens=y["cu"], max_tokens=y["most"])
+
+        out = run()
+        pg.check_attention(out, y)
+        assert torch.equal(out, run())
+    assert _status(b200) == 0
