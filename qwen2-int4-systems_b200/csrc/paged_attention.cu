@@ -674,14 +674,20 @@ cudaError_t launch_kernel(int D, bool f16, int nt, const CUtensorMap& k, const C
   return f16 ? launch_rows<64, true>(nt, k, v, a, ctas, s) : launch_rows<64, false>(nt, k, v, a, ctas, s);
 }
 
-// Rows of one sequence and KV head from which the tcgen05 kernel takes a batch
-// (its tiles hold whole tokens, and its row maxima want a scale that is not
-// negative). Beyond 32 rows mma.sync would take several tiles and read the keys
-// for each: 48 rows over 1000 keys of a shared prefix 30.7 us by mma.sync, 24.4
-// by tcgen05 (both with the suffix's launches of then); 20 rows of each of 24
-// ragged sequences of up to 6005 keys 36.6 and 50.5.
-constexpr int64_t kTcFrom = 33;
-bool takes_tc(int64_t tokens, int64_t G, float scale) { return tokens * G >= kTcFrom && G <= 128 && scale >= 0.f; }
+// Whether a batch of up to `tokens` per sequence goes to the tcgen05 kernel (its
+// tiles hold whole tokens, and its row maxima want a scale that is not
+// negative): by the rows of a sequence and KV head. Beyond 32 mma.sync would
+// take several tiles and read the keys for each (48 rows over 1000 keys of a
+// shared prefix 30.7 us by mma.sync, 24.4 by tcgen05, both with the suffix's
+// launches of then); with 128 dims its tile of 32 rows does not fit the
+// registers. mma.sync and tcgen05, us, 64 sequences of 2000 keys, 2 KV heads of
+// 128 dims: 24 rows 46.8 and 49.5, 28 rows 84.0 and 49.7, 32 rows 83.8 and 49.0
+// (one sequence of 300 keys: 8.9 and 13.3, 13.0 and 13.3, 13.2 and 13.1); of 64
+// dims: 24 rows 26.6 and 40.3, 32 rows 31.7 and 39.5.
+int64_t tc_from(int D) { return D == 128 ? 25 : 33; }
+bool takes_tc(int64_t tokens, int64_t G, int D, float scale) {
+  return tokens * G >= tc_from(D) && G <= 128 && scale >= 0.f;
+}
 
 // Where the tables cover at most this many keys, an item is one CTA's work and
 // no joining launch follows; half as many for mma.sync items that are fewer
@@ -699,7 +705,7 @@ constexpr int kWholeKeys = 512;
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 // Room for the pieces of a launch over `tokens` per sequence, and what the runs note of their split items.
 size_t pieces_bytes(int64_t tokens, int64_t G, int D, int ctas) {
-  const size_t rows = takes_tc(tokens, G, 1.f) ? kTcRows : 32;
+  const size_t rows = takes_tc(tokens, G, D, 1.f) ? kTcRows : 32;
   return round256((size_t)ctas * (2 * rows * (D + 2) * sizeof(float) + sizeof(SplitItem)));
 }
 size_t state_bytes(int64_t T, int64_t Hq, int D) { return (size_t)(T * Hq) * (D + 2) * sizeof(float); }
@@ -776,7 +782,7 @@ int attend(const Call& c, const char* what) {
   // Units are counted in 32 bits (paged_attention.cuh): tiles of the batch times units of the longest item.
   {
     auto units = [&](int64_t tokens, int64_t seqs, int64_t per_seq, int64_t keys) {
-      const int64_t rows = takes_tc(per_seq, G, c.scale) ? kTcRows / 2 : 8;
+      const int64_t rows = takes_tc(per_seq, G, D, c.scale) ? kTcRows / 2 : 8;
       return (double)(tokens * G / rows + seqs) * kv.kv_heads * (keys / kBlockKeys + 2);
     };
     if (units(c.T, c.B, most, (int64_t)kv.table_width * kv.page_size) >= 2147483647.0 ||
@@ -799,7 +805,7 @@ int attend(const Call& c, const char* what) {
   CUtensorMap qmap, kmap, vmap;
   const uint32_t box_rows = (uint32_t)std::min(kv.page_size, kBlockKeys);
   if (!tensor_map_pages(&kmap, kv.k, kv, box_rows) || !tensor_map_pages(&vmap, kv.v, kv, box_rows)) return QI4_ERR_LAUNCH;
-  if (takes_tc(prefix ? c.T : most, G, c.scale) &&
+  if (takes_tc(prefix ? c.T : most, G, D, c.scale) &&
       !tensor_map_rows3(&qmap, c.q, kv.dtype == QI4_DTYPE_F16, D, c.Hq, c.T, c.q_head, c.q_tok, (uint32_t)G,
                         (uint32_t)(kTcRows / G)))
     return QI4_ERR_LAUNCH;
@@ -824,10 +830,10 @@ int attend(const Call& c, const char* what) {
   cudaError_t e = cudaSuccess;
   // One launch: pieces at `at`, the kernel for `tokens` per sequence. The
   // mma.sync tile is the smallest of 8, 16, 24 and 32 rows that holds them (the
-  // 20 rows named at kTcFrom: 36.6 us in tiles of 24, 44.6 in tiles of 32).
+  // 20 rows of each of 24 ragged sequences of up to 6005 keys, 64 dims: 36.6 us in tiles of 24, 44.6 in tiles of 32).
   auto launch = [&](PagedArgs& x, char* at, int64_t tokens) {
-    const bool tc = takes_tc(tokens, G, c.scale);
-    const size_t rows = takes_tc(tokens, G, 1.f) ? kTcRows : 32;
+    const bool tc = takes_tc(tokens, G, D, c.scale);
+    const size_t rows = takes_tc(tokens, G, D, 1.f) ? kTcRows : 32;
     x.ws = reinterpret_cast<float*>(at);
     const int R = tc ? kTcRows : tokens * G <= 8 ? 8 : tokens * G <= 16 ? 16 : tokens * G <= 24 ? 24 : 32;
     x.tile_tokens = (int)(R / G);
