@@ -28,9 +28,9 @@
 //             and values by turns (128-byte swizzle throughout).
 // The weights of a unit are announced in two halves of 64 keys, so that the
 // first half's product runs under the second half's exponentials. (Scores in
-// halves of 64 columns as well, to have one half's always ready, took longer:
-// a product of N = 64 with both operands in shared memory takes the 64 cycles
-// of one with N = 128.)
+// halves of 64 columns as well, to have one half's always ready, took longer
+// with one warp for the products: they are twice as many, and with N = 64 and
+// both operands in shared memory each takes 48 cycles against 64 with N = 128.)
 // Tensor memory: scores 2 x 128 columns, sums 2 x D. All waits are bounded.
 //
 // Measured (device time, BF16, 12 query heads on 2 KV heads of 128 dims): a
@@ -38,12 +38,14 @@
 // tokens 111 us. A unit takes some 4000 cycles: the tensor cores are active for
 // 46% of them and the exponentials' pipe as long. Neither alone is the bound
 // (230 us become 198 without the exponentials, 213 with an eighth of the
-// products): it is the chain scores - maximum - weights - product of either
-// tile, whose turns interlock only in part. Slower were: the maximum and the
+// products): it is the chain scores - maximum - weights - product of a tile,
+// which one tile alone takes as long for. Slower were: the maximum and the
 // weights of a whole unit at once (288 us; 276 with registers moved from the
 // other warps), 16 softmax warps of half a row each (313), a warp for the
-// products of either tile (248), products issued by the softmax warps (266 to
-// 248 then), weights under the old maximum beside the search for the new (241).
+// products of either tile (248; with scores in halves of 64 keys, always one
+// ready, 230, and a quarter of the exponentials as polynomials then 225),
+// products issued by the softmax warps (266 to 248 then), weights under the old
+// maximum beside the search for the new (241).
 #include <atomic>
 
 #include "paged_attention.cuh"
