@@ -23,8 +23,9 @@
 // further unit 6 to 7 TB/s, so what bounds them is the 9 to 11 us of a call
 // that do not grow with the keys: the launch, each warp's way to its first unit
 // (boundaries, lengths and page table, one after the other), the warps' sums,
-// the joining launch. Few items of tables that cover up to 4096 keys are a
-// cluster's work each, without a joining launch: one sequence of 641 keys 6.3 us.
+// the joining launch. Items that leave two CTAs or more for each, of tables that
+// are not long, are a cluster's work, without a joining launch: one sequence of
+// 641 keys 6.3 us, 16 of 450 keys 6.3.
 // Sixteen consumer warps in two groups that take the units
 // by turns had 96 registers each and were slower (25.1 us for the 64).
 #include <cooperative_groups.h>
@@ -448,14 +449,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = (int)cluster.block_rank() * kThreads + threadIdx.x; i < rows * kLanes; i += C * kThreads) {
       const int r = i / kLanes, d = (i - r * kLanes) * 4;
       float acc[4] = {0.f, 0.f, 0.f, 0.f}, top = -INFINITY, sum = 0.f;
-      for (int p0 = 0; p0 < C; p0 += 8) {  // (clusters are of 8 or 16)
+      for (int p0 = 0; p0 < C; p0 += 8) {
         float2 ml[8];
         float4 v[8];
 #pragma unroll
         for (int p = 0; p < 8; ++p) {
-          const float* there = cluster.map_shared_rank(part, p0 + p);
-          ml[p] = *reinterpret_cast<const float2*>(there + R * D + 2 * r);
-          v[p] = *reinterpret_cast<const float4*>(there + r * D + d);
+          ml[p] = make_float2(-INFINITY, 0.f);
+          if (p0 + p < C) {
+            const float* there = cluster.map_shared_rank(part, p0 + p);
+            ml[p] = *reinterpret_cast<const float2*>(there + R * D + 2 * r);
+            v[p] = *reinterpret_cast<const float4*>(there + r * D + d);
+          }
         }
         float to = top;
 #pragma unroll
@@ -588,14 +592,30 @@ int read_paged_error(cudaStream_t stream) { return read_error_word(&g_paged_erro
 
 namespace {
 
-// Keys that a table may cover for few items (at most as many as clusters of
-// their CTAs are resident at once) to be the work of a cluster each: one
-// launch, no pieces in memory. Dealt to all SMs and in clusters, us (12 query
-// heads on 2 KV heads of 128 dims): one sequence of 641 keys 8.4 and 6.3, of
-// 4000 8.9 and 8.0; four of 1000 9.0 and 6.3, of 4000 10.6 and 10.4; beyond, the
-// cluster's SMs would be the bound. Clusters of 16 CTAs where the tables cover
-// more than 8 units and so many are resident (2000 keys: one sequence 6.7, four
-// in clusters of 8 7.5), else of 8 (one sequence of 1000 keys 6.1, of 16 6.6).
+// Where the tables cover at most this many keys, an item is one CTA's work and
+// no joining launch follows; half as many for mma.sync items that leave two
+// CTAs or more for each (clusters take those). Lengths are on the device: the
+// tables' width is what the host knows. Split and whole, us: 64 sequences of 500
+// keys, 12 query heads on 2 KV heads of 128 dims 15.3 and 12.0; 1 sequence of
+// 250 keys 8.5 and 7.1, of 500 8.4 and 9.9; 16 prompts of 500 tokens 42.5 and
+// 37.1, 1 prompt of 200 16.4 and 13.3, of 500 18.1 and 17.6. More keys are split
+// although even batches would still gain (64 sequences of 1000 keys: 20.7 and
+// 18.0), for the sake of batches with one long sequence among short ones (alone
+// at 1000 keys: 8.6 and 15.8). A shared prefix, few long items of one length, is
+// always split (500 keys under 64 sequences: 23.1 and 27.6).
+constexpr int kWholeKeys = 512;
+
+// Where no more items of one row tile are in a batch than clusters of 16, 8, 4
+// or 2 CTAs are resident at once, an item is the work of one cluster, the
+// largest such, if the tables cover at most kWholeKeys for each of its CTAs and
+// kClusterKeys in all: one launch, no pieces in memory. Dealt to all SMs and in
+// clusters, us (12 query heads on 2 KV heads of 128 dims): one sequence of 641
+// keys 8.4 and 6.3, of 4000 8.9 and 8.0; four of 1000 9.0 and 6.3, of 4000 10.6
+// and 10.4; 16 of 450 10.3 and 6.3, of 2000 14.3 and 11.1; 32 of 900 14.0 and
+// 10.4; ragged, 8 of up to 4000 10.7 and 10.6, 32 of up to 1000 10.4 and 9.7.
+// Clusters of 16 only where the tables cover more than 8 units (one sequence of
+// 1000 keys: 6.1 in a cluster of 8 and 6.7 of 16; of 2000: 6.7 of 16, four of
+// them in clusters of 8 7.5).
 constexpr int kClusterKeys = 4096;
 
 template <int D, int NT, bool F16, bool kClusters>
@@ -626,16 +646,16 @@ cudaError_t launch_decode(const CUtensorMap& k, const CUtensorMap& v, const Page
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   const int64_t items = (int64_t)a.r.B * a.Hkv;
-  if (a.one_tile && !a.unsplit && a.cap <= kClusterKeys && items * 8 <= ctas) {
-    // Clusters that are all resident at once: of 8 CTAs, or of 16 where the tables cover more units than 8.
+  if (a.one_tile && !a.unsplit && a.cap <= kClusterKeys && items * 2 <= ctas) {
     auto kernel = paged_decode_kernel<D, NT, F16, true>;
     cudaError_t e = configure<D, NT, F16, true>(dev);
     if (e != cudaSuccess) return e;
-    static std::atomic<int> resident[2][64];  // clusters of 16 and of 8 on a device, plus one
+    static std::atomic<int> resident[4][64];  // clusters of 16, 8, 4 and 2 on a device, plus one
     cfg.dynamicSmemBytes = smem_of(D, NT, true);
     cfg.numAttrs = 2;
-    for (int i = a.cap > 8 * kBlockKeys ? 0 : 1; i < 2; ++i) {
+    for (int i = a.cap > 8 * kBlockKeys ? 0 : 1; i < 4; ++i) {
       const int C = 16 >> i;
+      if (a.cap > C * kWholeKeys) break;
       attr[1].val.clusterDim.x = (unsigned)C;
       cfg.gridDim = dim3((unsigned)(items * C), 1, 1);
       int fit = resident[i][dev & 63].load(std::memory_order_relaxed) - 1;
@@ -688,19 +708,6 @@ int64_t tc_from(int D) { return D == 128 ? 25 : 33; }
 bool takes_tc(int64_t tokens, int64_t G, int D, float scale) {
   return tokens * G >= tc_from(D) && G <= 128 && scale >= 0.f;
 }
-
-// Where the tables cover at most this many keys, an item is one CTA's work and
-// no joining launch follows; half as many for mma.sync items that are fewer
-// than half the CTAs. Lengths are on the device: the tables' width is what the
-// host knows. Split and whole, us: 64 sequences of 500 keys, 12 query heads on
-// 2 KV heads of 128 dims 15.3 and 12.0; 1 sequence of 250 keys 8.5 and 7.1, of
-// 500 8.4 and 9.9; 16 prompts of 500 tokens 42.5 and 37.1, 1 prompt of 200 16.4
-// and 13.3, of 500 18.1 and 17.6. More keys are split although even batches
-// would still gain (64 sequences of 1000 keys: 20.7 and 18.0), for the sake of
-// batches with one long sequence among short ones (alone at 1000 keys: 8.6 and
-// 15.8). A shared prefix, few long items of one length, is always split (500
-// keys under 64 sequences: 23.1 and 27.6).
-constexpr int kWholeKeys = 512;
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 // Room for the pieces of a launch over `tokens` per sequence, and what the runs note of their split items.
@@ -842,7 +849,7 @@ int attend(const Call& c, const char* what) {
     x.by_tile_rows = FastDiv::of(x.tile_rows);
     x.by_G = FastDiv::of(G);
     x.by_ctas = FastDiv::of(sms);
-    x.unsplit = !x.late && x.cap <= (tc || (int64_t)x.r.B * x.Hkv * 2 >= sms ? kWholeKeys : kWholeKeys / 2);
+    x.unsplit = !x.late && x.cap <= (tc || (int64_t)x.r.B * x.Hkv * 2 > sms ? kWholeKeys : kWholeKeys / 2);
     x.splits = reinterpret_cast<SplitItem*>(at + (size_t)sms * 2 * rows * (D + 2) * sizeof(float));
     if (tc) return launch_paged_tc(D, f16, qmap, kmap, vmap, x, sms, c.stream);
     return launch_kernel(D, f16, R / 8, kmap, vmap, x, sms, c.stream);

@@ -71,7 +71,8 @@ def b200_paged_attention(q, k_cache, v_cache, block_table, lengths, *, cu_tokens
     number: no sequence has more new tokens, which ``qi4_device_status``
     checks) lets a batch given by ``cu_tokens`` run on the kernel and the
     tiles for its row count. A block_table may be wider than the lengths need;
-    one that covers at most 512 keys (4096 for few sequences) saves a launch.
+    one that covers at most 512 keys (up to 4096 for few sequences) saves a
+    launch.
     ``workspace``: a uint8 tensor of ``qi4_paged_attention_workspace`` bytes,
     for callers that own their memory.
     """

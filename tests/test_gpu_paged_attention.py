@@ -299,3 +299,19 @@ def test_few_sequences_however_wide_the_table(b200, cuda_device, seqs, Hq, Hkv, 
         pg.check_attention(out, y)
         assert torch.equal(out, run())
     assert _status(b200) == 0
+
+
+@pytest.mark.parametrize("seqs,Hq,Hkv,D,page,pages,dtype", [
+    ([(1, 1 + 130 * i) for i in range(15)], 12, 2, 128, 16, 128, BF16),
+    ([(1 + i % 5, 1000 - 31 * i) for i in range(9)], 16, 4, 64, 8, 200, F16),
+    ([(i % 4, 11 * i) for i in range(31)], 8, 2, 128, 32, 32, F16),
+])
+def test_sequences_that_share_the_gpu_in_small_clusters(b200, cuda_device, seqs, Hq, Hkv, D, page, pages, dtype):
+    x = pg.build(seqs, Hq=Hq, Hkv=Hkv, D=D, page=page, dtype=dtype, device=cuda_device, wide=0)
+    table = torch.full((len(seqs), pages), -1, dtype=torch.int32, device=cuda_device)
+    table[:, :x["table"].shape[1]] = x["table"]
+    y = dict(x, table=table)
+    out = _run(b200, y, max_tokens=y["most"])
+    pg.check_attention(out, y)
+    assert torch.equal(out, _run(b200, y, max_tokens=y["most"]))
+    assert _status(b200) == 0
