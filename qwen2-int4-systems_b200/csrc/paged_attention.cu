@@ -600,9 +600,10 @@ namespace {
 // 250 keys 8.5 and 7.1, of 500 8.4 and 9.9; 16 prompts of 500 tokens 42.5 and
 // 37.1, 1 prompt of 200 16.4 and 13.3, of 500 18.1 and 17.6. More keys are split
 // although even batches would still gain (64 sequences of 1000 keys: 20.7 and
-// 18.0), for the sake of batches with one long sequence among short ones (alone
-// at 1000 keys: 8.6 and 15.8). A shared prefix, few long items of one length, is
-// always split (500 keys under 64 sequences: 23.1 and 27.6).
+// 18.0), for the sake of ragged ones, whose longest sequence would be the bound
+// (64 of up to 1000 keys: 13.8 and 17.4; one of 1000 alone 8.6 and 15.8). A
+// shared prefix, few long items of one length, is always split (500 keys under
+// 64 sequences: 23.1 and 27.6).
 constexpr int kWholeKeys = 512;
 
 // Where no more items of one row tile are in a batch than clusters of 16, 8, 4
