@@ -45,7 +45,9 @@ bool tensor_map_pages(CUtensorMap* out, const void* base, const qi4_paged_kv& kv
 bool tensor_map_rows3(CUtensorMap* out, const void* base, bool f16, int64_t dims, int64_t heads, int64_t rows,
                       int64_t head_stride, int64_t row_stride, uint32_t box_heads, uint32_t box_rows);
 
-// Device-side error flags (one per translation unit), read and cleared on host.
+// Device-side error flags (one word per translation unit), read and cleared on
+// host. A word may hold reports of a call's inputs (QI4_DEVICE_*) beside this
+// bit, which alone says that a wait ran out.
 constexpr int kErrWaitTimeout = 1;
 
 // ---------------------------------------------------------------------------
@@ -128,8 +130,10 @@ __device__ __forceinline__ bool mbar_wait_for(uint64_t* bar, uint32_t parity, in
     // A wait that already timed out somewhere means the pipeline is broken:
     // give up instead of queueing further time-outs. (Checked here, not
     // before the first spin, so that an ordinary short wait never pays a
-    // global-memory round trip.)
-    if (*reinterpret_cast<volatile int*>(err) != 0) return false;
+    // global-memory round trip.) The word's other bits report inputs and say
+    // nothing about the pipeline: a wait that gave up for one of them would
+    // let its data be read before it is there.
+    if (*reinterpret_cast<volatile int*>(err) & kErrWaitTimeout) return false;
     if (global_timer_ns() - start > limit_ns) break;
   }
   atomicOr(err, kErrWaitTimeout);
