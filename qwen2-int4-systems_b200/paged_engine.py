@@ -61,6 +61,12 @@ def random_decoder(config, *, device="cuda", seed: int = 0):
                            model=SimpleNamespace(embed_tokens=embed, layers=layers, norm=norm()))
 
 
+def _owners(cu_tokens, t):
+    """The sequence of each of the tokens t; tokens behind the last sequence's, whose results are not defined, count as
+    that one's, so that they index nothing beyond the batch."""
+    return torch.searchsorted(cu_tokens[1:], t, right=True).clamp_max(cu_tokens.numel() - 2)
+
+
 class PagedDecoder:
     """``batch`` sequences of up to ``max_len`` keys each (a shared prefix not counted) in pages of ``page_size``."""
 
@@ -133,7 +139,7 @@ class PagedDecoder:
         positions = None
         if self.prefix_len:  # rotary positions run on from the prefix's
             t = torch.arange(T, device=self.device)
-            owner = t // max(max_tokens, 1) if cu_tokens is None else torch.searchsorted(cu_tokens[1:], t, right=True)
+            owner = t // max(max_tokens, 1) if cu_tokens is None else _owners(cu_tokens, t)
             positions = (self.prefix_len + before[owner] + t - first[owner]).to(torch.int32)
 
         def append(q, k, v, kc, vc):
