@@ -209,6 +209,9 @@ def speculative_generate(target: PagedDecoder, draft: PagedDecoder, prompts, max
         for model in (target, draft):
             model.forward(body, cu_tokens=cu, max_tokens=longest - 1)
     last = torch.stack([p[-1] for p in prompts]).to(dev)
+    # Where the caches end with all but the last returned token. A sequence may go beyond it by `drafts` as it finishes;
+    # it is taken back to it, so that what later steps still append to it needs no more room than an open sequence's.
+    end_t, end_d = target.lengths + max_new_tokens, draft.lengths + max_new_tokens
 
     def probs(model, hidden):
         return torch.softmax(model.logits(hidden).float() / temperature, dim=-1)
@@ -238,7 +241,8 @@ def speculative_generate(target: PagedDecoder, draft: PagedDecoder, prompts, max
         out.scatter_(1, torch.where(open_[:, None], made[:, None] + place, out.shape[1] - 1), found)
         last = torch.where(open_, found.gather(1, accepted.long()[:, None])[:, 0], last)
         made += step
-        target.lengths, draft.lengths = ((s + step).to(torch.int32) for s in (start_t, start_d))
+        target.lengths = torch.minimum(start_t + step, end_t).to(torch.int32)
+        draft.lengths = torch.minimum(start_d + step, end_d).to(torch.int32)
         stood += int(accepted[open_].sum())
         tried += drafts * int(open_.sum())
     return out[:, :max_new_tokens], stood / max(tried, 1)
