@@ -465,7 +465,7 @@ QI4_API int qi4_paged_attention(const qi4_paged_kv* kv, const void* q, int64_t q
 
 /*
  * The same for a batch whose sequences all begin with one prefix of
- * prefix_length cached keys in the pages prefix_table[0 .. prefix_pages) of
+ * prefix_length cached keys (at most 2^30) in the pages prefix_table[0 .. prefix_pages) of
  * the same pool: every token sees all of the prefix and, causally, its own
  * sequence's lengths[b] further keys (block_table covers these alone). The
  * prefix is read once for the whole batch. The workspace is that of

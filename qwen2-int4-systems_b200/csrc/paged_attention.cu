@@ -779,7 +779,12 @@ int attend(const Call& c, const char* what) {
     set_error("%s: a prefix needs its page table and a length that is not negative", what);
     return QI4_ERR_ARGUMENT;
   }
-  if (prefix && c.prefix_len > c.prefix_width * kv.page_size) {
+  if (c.prefix_len > (1ll << 30)) {
+    set_error("%s: a prefix has at most 2^30 keys (got %lld)", what, (long long)c.prefix_len);
+    return QI4_ERR_SHAPE;
+  }
+  const int64_t prefix_pages = (c.prefix_len + kv.page_size - 1) / kv.page_size;  // of the table, those that are read
+  if (prefix && prefix_pages > c.prefix_width) {
     set_error("%s: the prefix is longer (%lld) than its page table covers", what, (long long)c.prefix_len);
     return QI4_ERR_SHAPE;
   }
@@ -867,7 +872,7 @@ int attend(const Call& c, const char* what) {
     a.state_acc = state, a.state_ml = state + c.T * c.Hq * D;
     e = launch(a, ws, most);
     PagedArgs p = a;
-    p.table = c.prefix_table, p.table_stride = 0, p.table_width = (int)c.prefix_width;
+    p.table = c.prefix_table, p.table_stride = 0, p.table_width = (int)prefix_pages;
     p.r = {nullptr, nullptr, 1, (int)c.T, (int)c.T};
     p.fixed_len = (int)c.prefix_len, p.cap = (int)c.prefix_len, p.causal = 0;
     p.prior_acc = a.state_acc, p.prior_ml = a.state_ml, p.late = 1;
