@@ -416,8 +416,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int x = 0; x < kWarps; ++x) top = fmaxf(top, rm[x * R + r]);
 #pragma unroll
-        for (int x = 0; x < kWarps; ++x)
-          sum += rm[x * R + r] == -INFINITY ? 0.f : rl[x * R + r] * exp2_approx(rm[x * R + r] - top);
+        for (int x = 0; x < kWarps; ++x)  // (a warp without a maximum has a sum of 0, or of NaN where no score is a number)
+          sum += rm[x * R + r] == -INFINITY ? rl[x * R + r] : rl[x * R + r] * exp2_approx(rm[x * R + r] - top);
         float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int x = 0; x < kBuffers; ++x) {
@@ -464,16 +464,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         float to = top;
 #pragma unroll
         for (int p = 0; p < 8; ++p) to = fmaxf(to, ml[p].x);
-        if (to == -INFINITY) continue;
-        const float back = exp2_approx(top - to);
+        const float base = to == -INFINITY ? 0.f : to, back = exp2_approx(top - base);
         top = to;
         sum *= back;
 #pragma unroll
         for (int k = 0; k < 4; ++k) acc[k] *= back;
 #pragma unroll
         for (int p = 0; p < 8; ++p) {
-          if (ml[p].x == -INFINITY) continue;  // (its sums may not have been written)
-          const float f = exp2_approx(ml[p].x - to);
+          // A piece that saw no key has written no sums. (One whose scores are no numbers has: its sum of weights is NaN.)
+          if (ml[p].x == -INFINITY && ml[p].y == 0.f) continue;
+          const float f = exp2_approx(ml[p].x - base);
           sum += ml[p].y * f;
           acc[0] += v[p].x * f, acc[1] += v[p].y * f, acc[2] += v[p].z * f, acc[3] += v[p].w * f;
         }
