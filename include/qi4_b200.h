@@ -449,13 +449,15 @@ QI4_API int qi4_rope_paged_append(const qi4_paged_kv* kv, const void* q, int64_t
  * scores, softmax and sums; the weights of the second product are carried to
  * 16 bits or more where a tile has few rows, and rounded to the cache's type
  * on the tcgen05 path (max_tokens * Hq / kv_heads large). What page slots
- * beyond a length hold does not matter, NaN included. q as in
+ * beyond a length hold does not matter, NaN included; keys and values that
+ * are not finite reach the tokens that see them, and no other. q as in
  * qi4_rope_paged_append, its strides positive; out [T, Hq, head_dim]
  * contiguous, 32-byte aligned; head_dim 64 or 128.
  * max_tokens: no sequence has more new tokens (0: not known); it chooses the
- * kernel and its tiles, and with the width of the block tables the work split. workspace: qi4_paged_attention_workspace bytes,
- * 16-byte aligned, no initialisation needed, not shared by calls that may
- * overlap; NULL: the library's scratch pool. Replaces, for a paged cache,
+ * kernel and its tiles, and with the width of the block tables the work
+ * split. workspace: qi4_paged_attention_workspace bytes, 16-byte aligned, no
+ * initialisation needed, not shared by calls that may overlap; NULL: the
+ * library's scratch pool. Replaces, for a paged cache,
  * reference src/qwen_int4/model.py:90-118.
  */
 QI4_API int qi4_paged_attention(const qi4_paged_kv* kv, const void* q, int64_t q_token_stride,
@@ -465,10 +467,10 @@ QI4_API int qi4_paged_attention(const qi4_paged_kv* kv, const void* q, int64_t q
 
 /*
  * The same for a batch whose sequences all begin with one prefix of
- * prefix_length cached keys (at most 2^30) in the pages prefix_table[0 .. prefix_pages) of
- * the same pool: every token sees all of the prefix and, causally, its own
- * sequence's lengths[b] further keys (block_table covers these alone). The
- * prefix is read once for the whole batch. The workspace is that of
+ * prefix_length cached keys (at most 2^30) in the pages prefix_table[0 ..
+ * prefix_pages) of the same pool: every token sees all of the prefix and,
+ * causally, its own sequence's lengths[b] further keys (block_table covers
+ * these alone). The prefix is read once for the whole batch. The workspace is that of
  * qi4_paged_attention_workspace with prefix = 1. No reference counterpart.
  */
 QI4_API int qi4_shared_prefix_attention(const qi4_paged_kv* kv, const void* q, int64_t q_token_stride,

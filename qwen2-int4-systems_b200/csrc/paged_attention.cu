@@ -50,7 +50,7 @@ constexpr int stage_bytes(int D) { return 2 * kBlockKeys * D * 2; }
 constexpr size_t smem_of(int D, int NT, bool clusters) {
   return 1024 + (size_t)stages_of(D) * stage_bytes(D) + (size_t)8 * NT * (2 * D + 16) +
          2 * 2 * kWarps * 8 * NT * sizeof(float) + 2 * stages_of(D) * sizeof(uint64_t) +
-         (clusters ? 8 * NT * (D + 2) * sizeof(float) : 0);
+         (clusters ? 8 * NT * (D + 2) * sizeof(float) : 0) + sizeof(int);
 }
 
 template <bool F16>
@@ -83,11 +83,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
   return d;
 }
-template <bool F16>
-__device__ __forceinline__ float2 unpack2(uint32_t w) {
-  if constexpr (F16) return __half22float2(*reinterpret_cast<const __half2*>(&w));
-  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
-}
 // kClusters: an item is the work of one cluster, whose CTAs share its units out
 // in order and exchange their sums over distributed shared memory; else the
 // units are dealt to all CTAs (paged_attention.cuh).
@@ -106,6 +101,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* full = reinterpret_cast<uint64_t*>(red_l + 2 * kWarps * R);
   uint64_t* empty = full + kStages;
   float* part = reinterpret_cast<float*>(empty + kStages);  // kClusters: [R][D] sums, [R] (max, sum)
+  int* odd = reinterpret_cast<int*>(part + (kClusters ? R * (D + 2) : 0));  // the last item with odd values to add
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -113,6 +109,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], kWarps);
     }
+    *odd = 0;
     fence_barrier_init();
     prefetch_tensor_map(&kmap);
     prefetch_tensor_map(&vmap);
@@ -184,8 +181,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int gq = lane >> 2, tq = lane & 3;
   const int r0 = warp * 16;  // this warp's keys of every unit
   const int lrow = r0 + (lane & 7) + (((lane >> 3) & 1) << 3), lchunk = lane >> 4, lx = lane & 7;
-  int par = 0;
+  int par = 0, item = 0;
   for (bool one = warp < kWarps; kClusters ? one : w.next(a); one = false) {
+    ++item;
     const int rows = w.rows(a), vis = w.tile_visible(a), nload = w.loaded(vis);
     if (kClusters && nload == 0) {
       if (threadIdx.x < R) *reinterpret_cast<float2*>(part + R * D + 2 * threadIdx.x) = make_float2(-INFINITY, 0.f);
@@ -245,14 +243,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t kb = smem_addr(smem + stage * kStageBytes) + lrow * 128;
         const uint32_t vb = kb + (D / 64) * kHalfBytes;
         if (key0 < vis) {
-          if (key0 + 16 > vis) {
+          if (key0 + 16 > lim_min) {
             // Slots past the last key may hold anything: their values are
-            // zeroed, as a weight of zero times a NaN is not zero.
+            // zeroed, as a weight of zero times a NaN is not zero. So are the
+            // odd ones of keys that not every row sees.
             for (int j = lane; j < 16 * (D / 8); j += 32) {
               const int r = j / (D / 8), ch = j - r * (D / 8);
               if (key0 + r >= vis)
                 sts128(smem_addr(smem + stage * kStageBytes) + (D / 64 + (ch >> 3)) * kHalfBytes + (r0 + r) * 128 +
                            ((ch & 7) << 4), make_uint4(0u, 0u, 0u, 0u));
+            }
+            const int some = min(16, vis - key0) * (D / 8);
+#pragma unroll 1
+            for (int j = max(0, lim_min - key0) * (D / 8) + lane; j < some; j += 32) {
+              const int r = j / (D / 8), ch = j - r * (D / 8);
+              if (clear_odd<F16>(smem_addr(smem + stage * kStageBytes) + (D / 64 + (ch >> 3)) * kHalfBytes +
+                                 (r0 + r) * 128 + ((ch & 7) << 4)))
+                atomicMax(odd, item);
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -431,6 +438,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         } else {
           *reinterpret_cast<float4*>(slot + r * D + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
           if (d == 0) *reinterpret_cast<float2*>(slot + R * D + 2 * r) = make_float2(top, sum);
+        }
+      }
+      if (*static_cast<volatile int*>(odd) >= item) {  // (written before the barriers above)
+#pragma unroll 1
+        for (int i = threadIdx.x; i < rows * kLanes; i += 32 * kWarps) {
+          const int r = i / kLanes, d = (i - r * kLanes) * 4;
+          int token, head;
+          w.place(a, r, token, head);
+          const int64_t row = (int64_t)token * (a.Hkv * a.G) + head;
+          add_odd<F16>(a, w.b, w.kvh, max(lim_min, w.blk * kBlockKeys),
+                       min(w.row_visible(a, r), (w.blk + nload) * kBlockKeys), d, 4, a.out + row * D,
+                       !whole ? slot + r * D : a.state_acc ? a.state_acc + row * D : nullptr, 1);
         }
       }
       fence_proxy_async_smem();
@@ -837,6 +856,8 @@ int attend(const Call& c, const char* what) {
   a.out = static_cast<uint16_t*>(c.out);
   a.page_shift = __builtin_ctz((unsigned)kv.page_size), a.box_shift = __builtin_ctz(box_rows);
   a.pages = kv.pages;
+  a.v = static_cast<const uint16_t*>(kv.v);
+  a.v_page = kv.page_stride, a.v_head = kv.head_stride, a.v_slot = kv.slot_stride;
   a.Hkv = kv.kv_heads, a.G = (int)(c.Hq / kv.kv_heads);
   a.scale_log2 = c.scale * 1.4426950408889634f;
   const bool f16 = kv.dtype == QI4_DTYPE_F16;

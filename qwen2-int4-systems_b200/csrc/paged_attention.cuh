@@ -32,6 +32,8 @@ struct PagedArgs {
   const int32_t* table;
   int64_t table_stride;
   int table_width, pages, page_shift, box_shift;  // box: rows of one copy, min(page_size, kBlockKeys)
+  const uint16_t* v;  // the values' pool, for add_odd
+  int64_t v_page, v_head, v_slot;
   Ragged r;
   int fixed_len;  // >= 0: every sequence has this many keys (lengths is not read)
   int Hkv, G, cap;
@@ -305,6 +307,12 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+template <bool F16>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if constexpr (F16) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+
 // Two floats rounded to the packed 16-bit type (lo in the low half).
 template <bool F16>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -314,6 +322,56 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   else
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
   return d;
+}
+
+// Values that are not finite (odd ones) at keys that only some rows of a tile
+// see: the product would make 0 x inf = NaN of them in the rows that do not. The
+// units that hold such keys (the last ones of a causal tile with several tokens)
+// have their odd values cleared before the product, and at the item's end the
+// rows that see them take them up from the pool: a positive weight times an
+// infinity or NaN is it, whatever the weight. Looking costs what these units'
+// batches take longer by: drafts (24 sequences, 20 rows each) 36.5 -> 37.7 us,
+// ragged chunks 112 -> 115, a prompt of 8192 tokens 248 -> 250.
+
+// Bits 15 and 31: that half of w is infinite or NaN.
+template <bool F16>
+__device__ __forceinline__ uint32_t odd_halves(uint32_t w) {
+  return ((w & (F16 ? 0x7C007C00u : 0x7F807F80u)) + (F16 ? 0x04000400u : 0x00800080u)) & 0x80008000u;
+}
+// Clears the odd ones of eight values in shared memory; whether there were any.
+template <bool F16>
+__device__ __forceinline__ bool clear_odd(uint32_t saddr) {
+  uint4 v = lds128(saddr);
+  const uint32_t x = odd_halves<F16>(v.x), y = odd_halves<F16>(v.y), z = odd_halves<F16>(v.z), w = odd_halves<F16>(v.w);
+  if (!(x | y | z | w)) return false;
+  v.x &= ~((x >> 15) * 0xFFFFu);
+  v.y &= ~((y >> 15) * 0xFFFFu);
+  v.z &= ~((z >> 15) * 0xFFFFu);
+  v.w &= ~((w >> 15) * 0xFFFFu);
+  sts128(saddr, v);
+  return true;
+}
+// Adds the odd values of keys from .. to - 1 of sequence b to what this thread has written for a row: its dims
+// d .. d + n - 1, FP32 at sums[dim * step], or the output where sums is null.
+template <bool F16>
+__device__ __forceinline__ void add_odd(const PagedArgs& a, int b, int kvh, int from, int to, int d, int n,
+                                        uint16_t* out, float* sums, int step) {
+#pragma unroll 1
+  for (int key = from; key < to; ++key) {
+    const int page = __ldg(a.table + b * a.table_stride + (key >> a.page_shift));
+    if (page < 0 || page >= a.pages) continue;  // (reads as zeros)
+    const uint16_t* v = a.v + page * a.v_page + kvh * a.v_head + (key & ((1 << a.page_shift) - 1)) * a.v_slot;
+#pragma unroll 1
+    for (int i = d; i < d + n; ++i) {
+      const uint32_t w = __ldg(v + i);
+      if (!odd_halves<F16>(w)) continue;
+      const float x = unpack2<F16>(w).x;
+      if (sums)
+        sums[i * step] += x;
+      else
+        out[i] = (uint16_t)pack2<F16>(unpack2<F16>(out[i]).x + x, 0.f);
+    }
+  }
 }
 
 // N dims (at d) of a finished row: weighted sums, max and sum of weights over

@@ -145,6 +145,21 @@ __host__ __device__ constexpr uint32_t idesc(bool f16, int N, bool v) {
          ((uint32_t)(128 >> 4) << 24);
 }
 
+// Clears the odd values of a key's row (chunks in an order by which neighbouring rows r meet in no bank).
+template <int D, bool F16>
+__device__ __forceinline__ bool clear_row(uint32_t row, int half_bytes, int r) {
+  uint32_t any = 0;
+#pragma unroll
+  for (int k = 0; k < D / 8; ++k) {
+    const uint4 v = lds128(row + (k >> 3) * half_bytes + ((k ^ r) & 7) * 16);
+    any |= odd_halves<F16>(v.x) | odd_halves<F16>(v.y) | odd_halves<F16>(v.z) | odd_halves<F16>(v.w);
+  }
+  if (!any) return false;
+#pragma unroll 1
+  for (int k = 0; k < D / 8; ++k) clear_odd<F16>(row + (k >> 3) * half_bytes + (k & 7) * 16);
+  return true;
+}
+
 template <int D, bool F16>
 __global__ void __launch_bounds__(kThreads, 1)
     paged_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
@@ -164,6 +179,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* kv_full = o_full + 2;                                              // [kSlots] TMA
   uint64_t* kv_empty = kv_full + kSlots;                                       // [kSlots] commit
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kv_empty + kSlots);
+  int* odd = reinterpret_cast<int*>(tmem_slot + 1);  // the last piece with odd values to add
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -179,6 +195,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&kv_full[i], 1);
       mbar_init(&kv_empty[i], 1);
     }
+    *odd = 0;
     fence_barrier_init();
     prefetch_tensor_map(&qmap);
     prefetch_tensor_map(&kmap);
@@ -316,10 +333,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     // The row maximum is taken of the raw scores (the scale is not negative here; never zero, which would make
     // a hidden key's -inf a NaN).
     const float scale = fmaxf(a.scale_log2, 1e-30f);
-    int pos = 0;
+    int pos = 0, item = 0;
     uint32_t ns = 0, no = 0, done = 0;  // uses of s_full, o_full, and o_done
     bool have = any && w.next(a);
     while (have) {
+      ++item;
       const int rows = w.rows(a), vis = w.tile_visible(a), nload = w.loaded(vis);
       const int base_pos = pos;
       pos += 2 * nload;
@@ -332,10 +350,27 @@ __global__ void __launch_bounds__(kThreads, 1)
       int token = 0, head = 0;
       if (live) w.place(a, row, token, head);
       const int lim = live ? w.row_visible(a, row) : 0, blk0 = w.blk;
+      const int lim_min = min(vis, w.row_visible(a, 0));  // the tile's first token sees the fewest keys
+      const int seq = w.b, kvh = w.kvh;
       float m = -INFINITY, l = 0.f;
       for (int h = 0; h < 2 * nload; ++h) {  // halves of 64 keys
         const int x = h & 1, key0 = (blk0 + (h >> 1)) * kBlockKeys + 64 * x;
         const uint32_t s_at = s_tm + 64 * x;
+        if (t == 0 && x == 0 && key0 + kBlockKeys > lim_min) {
+          // Slots past the last key may hold anything: their values are zeroed, as a weight of zero times a NaN is
+          // not zero. So are the odd ones of keys that not every row sees. (Here, while the scores are on their way:
+          // behind the weights it is on the path from one unit to the next: 8192 tokens 257 us against 250.)
+          const int vp = base_pos + h + 1, st = vp % kSlots;
+          mbar_wait(&kv_full[st], (uint32_t)(vp / kSlots) & 1u, &g_paged_tc_error);
+          const uint32_t at = smem_addr(ring + st * kSlotBytes) + r * 128;
+          if (key0 + r >= vis) {
+#pragma unroll
+            for (int k = 0; k < D / 8; ++k) sts128(at + (k >> 3) * kHalf + (k & 7) * 16, make_uint4(0u, 0u, 0u, 0u));
+          } else if (key0 + r >= lim_min && clear_row<D, F16>(at, kHalf, r)) {
+            atomicMax(odd, item);
+          }
+          fence_proxy_async_smem();
+        }
         if (x == 0) mbar_wait(&s_full[t], ns++ & 1u, &g_paged_tc_error);
         tc_fence_after();
         float s[64];
@@ -393,18 +428,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_st16(s_at + 16 * c, p);
         }
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        if (t == 0 && x == 0 && key0 + kBlockKeys > vis) {
-          // Slots past the last key may hold anything: their values are zeroed, as a weight of zero times a NaN is
-          // not zero.
-          const int vp = base_pos + h + 1, st = vp % kSlots;
-          mbar_wait(&kv_full[st], (uint32_t)(vp / kSlots) & 1u, &g_paged_tc_error);
-          if (key0 + r >= vis) {
-            const uint32_t at = smem_addr(ring + st * kSlotBytes) + r * 128;
-#pragma unroll
-            for (int k = 0; k < D / 8; ++k) sts128(at + (k >> 3) * kHalf + (k & 7) * 16, make_uint4(0u, 0u, 0u, 0u));
-          }
-          fence_proxy_async_smem();
-        }
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
@@ -438,6 +461,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (live && !whole) *reinterpret_cast<float2*>(slot + kTcRows * D + 2 * row) = make_float2(m, l);
+      // (Tile 1 sees the word too: the products behind its sums were issued after tile 0 had announced its weights.)
+      if (live && *static_cast<volatile int*>(odd) >= item) {
+        const int64_t at = (int64_t)token * (a.Hkv * a.G) + head;
+        add_odd<F16>(a, seq, kvh, max(lim_min, blk0 * kBlockKeys), min(lim, (blk0 + nload) * kBlockKeys), 0, D,
+                     a.out + at * D, !whole ? slot + row : a.state_acc ? a.state_acc + at * D : nullptr,
+                     whole ? 1 : kTcRows);
+      }
       tc_fence_before();  // the sums are read before the next item's first weights are announced
     }
   }

@@ -105,3 +105,26 @@ def test_keys_that_are_all_nan(b200, cuda_device, way):
     rows = _rows(x, 0)
     assert bool(got[rows].isnan().all())
     _check_but(got, x, rows)
+
+
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("way", WAYS)
+def test_a_value_reaches_no_token_that_does_not_see_its_key(b200, cuda_device, way, value):
+    """Values of new tokens, hidden from the tokens before them though in the same tile: w V with no weight for V is
+    not 0 x V. Those that see the key have the value's infinity, or NaN, in its dimension."""
+    x = _build(cuda_device, way)
+    v = x["v"].clone()
+    T, D = x["q"].shape[0], x["D"]
+    G = x["q"].shape[1] // x["Hkv"]
+    used = torch.zeros(T, x["q"].shape[1], D, dtype=torch.bool, device=cuda_device)
+    for b, (n, length) in enumerate(x["seqs"]):
+        for j, (i, d) in enumerate(((n - 1, 0), (n // 2, D - 1), (n // 2, 17), (1, 40))):
+            if 0 < i < n and length - n + i >= 0:
+                page, slot = _slot(x, b, length - n + i)
+                v[page, j % x["Hkv"], slot, d] = value
+                used[_rows(x, b, i), (j % x["Hkv"]) * G:(j % x["Hkv"] + 1) * G, d] = True
+    got = _run(b200, dict(x, v=v))
+    assert bool((got[used].isnan() if math.isnan(value) else got[used] == value).all())
+    assert bool(torch.isfinite(got[~used]).all())
+    ref, _ = pg.attention64(x)
+    pg.check_attention(torch.where(used, ref.to(got.dtype), got), x)
