@@ -447,10 +447,12 @@ QI4_API int qi4_rope_paged_append(const qi4_paged_kv* kv, const void* q, int64_t
  * appended before). causal: token i of n sees keys 0 .. lengths[b] - n + i;
  * else all lengths[b]. A token that sees no key has a zero output. FP32
  * scores, softmax and sums; the weights of the second product are carried to
- * 16 bits or more where a tile has few rows, and rounded to the cache's type
- * on the tcgen05 path (max_tokens * Hq / kv_heads large). What page slots
- * beyond a length hold does not matter, NaN included; keys and values that
- * are not finite reach the tokens that see them, and no other. q as in
+ * 16 bits (BF16) or 22 (FP16) where a tile has few rows, and rounded to the
+ * cache's type on the tcgen05 path (max_tokens * Hq / kv_heads, or the batch's
+ * tokens * Hq / kv_heads behind a prefix, from 25 rows of 128 dims or 33 of
+ * 64); in FP16 each is off by up to 2^-32 of its row's largest besides.
+ * What page slots beyond a length hold does not matter, NaN included; keys and
+ * values that are not finite reach the tokens that see them, and no other. q as in
  * qi4_rope_paged_append, its strides positive; out [T, Hq, head_dim]
  * contiguous, 32-byte aligned; head_dim 64 or 128.
  * max_tokens: no sequence has more new tokens (0: not known); it chooses the

@@ -313,6 +313,13 @@ __device__ __forceinline__ float2 unpack2(uint32_t w) {
   return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
 }
 
+// Weights are taken relative to 2^(max - kLift), sums of weights and of values alike. Against a row's maximum that lags
+// by up to 2^8 they reach 2^15 in FP16, which goes to 2^16, and not 2^8: FP16's steps end at 2^-24, so that a weight is
+// off by up to 2^-25 however small it is, 2^-32 of the largest one at least (it would be 2^-25 without the lift).
+// BF16 has FP32's exponents and needs none.
+template <bool F16>
+constexpr float kLift = F16 ? 7.f : 0.f;
+
 // Two floats rounded to the packed 16-bit type (lo in the low half).
 template <bool F16>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {

@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           m = to;
         }
-        const float nb = m == -INFINITY ? 0.f : -m;
+        const float nb = m == -INFINITY ? 0.f : kLift<F16> - m;
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
