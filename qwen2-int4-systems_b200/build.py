@@ -140,7 +140,10 @@ def build_torch_binding(force: bool = False) -> Path:
     """Compile csrc/*.cpp (the C++ side of the Python calls: the QuantLinear
     fast path and the paged-cache operators) against this interpreter's torch
     and libqi4_b200.so, in-tree next to the library. A source is recompiled
-    when it or the C header is newer than its object."""
+    when it or the C header is newer than its object; objects are kept per
+    compiler command and torch version (the command names the interpreter's
+    and torch's headers), and a module linked from others is linked anew."""
+    import hashlib
     import sysconfig
 
     import torch
@@ -163,20 +166,24 @@ def build_torch_binding(force: bool = False) -> Path:
         if proc.returncode != 0:
             raise RuntimeError(f"torch binding build failed:\n{proc.stderr[-4000:]}")
 
+    key = hashlib.sha256(" ".join([gxx, *flags, torch.__version__]).encode()).hexdigest()[:12]
+    stamp = BUILD / (out.name + ".key")  # what the module was linked from
     jobs, objects = [], []
     for src in sorted(CSRC.glob("*.cpp")):
-        obj = BUILD / (src.stem + ".cpp.o")
+        obj = BUILD / f"{src.stem}-{key}.cpp.o"
         objects.append(obj)
         if force or not obj.exists() or obj.stat().st_mtime < max(src.stat().st_mtime, header.stat().st_mtime):
             jobs.append(([gxx, *flags, "-c", str(src), "-o", str(obj)], BUILD / (src.stem + ".log")))
     if jobs:
         with ThreadPoolExecutor(max_workers=len(jobs)) as pool:
             list(pool.map(lambda j: run(*j), jobs))
-    if jobs or not out.exists() or out.stat().st_mtime < max(d.stat().st_mtime for d in [*objects, LIB]):
+    if (jobs or not out.exists() or not stamp.exists() or stamp.read_text() != key
+            or out.stat().st_mtime < max(d.stat().st_mtime for d in [*objects, LIB])):
         run([gxx, "-shared", *map(str, objects), "-o", str(out) + ".tmp", "-L", str(torch_dir / "lib"), "-ltorch",
              "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_cuda", "-L", str(PKG), "-lqi4_b200",
              "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + str(torch_dir / "lib")], BUILD / "torch_binding_link.log")
         os.replace(str(out) + ".tmp", out)
+        stamp.write_text(key)
     return out
 
 
