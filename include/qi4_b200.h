@@ -382,8 +382,9 @@ QI4_API int qi4_bf16_argmax_rows(const void* logits, int64_t B, int64_t V, int64
  *   slot * slot_stride (elements; V alike), head_dim contiguous elements.
  * Position p of sequence b lies in page block_table[b * table_stride +
  * p / page_size], slot p % page_size. page_size is a power of two from 8 to
- * 1024; k and v are 16-byte aligned, the strides multiples of 8 elements, so
- * [pages, heads, slots, dim] and [pages, slots, heads, dim] pools both fit.
+ * 1024; k and v are 16-byte aligned, the strides positive multiples of 8
+ * elements, so [pages, heads, slots, dim] and [pages, slots, heads, dim] pools
+ * both fit.
  *
  * A batch of B sequences brings T new tokens, the rows of [T, heads, dim]
  * tensors: sequence b owns rows cu_tokens[b] .. cu_tokens[b + 1] - 1 (device,
@@ -425,10 +426,11 @@ typedef struct qi4_paged_kv {
  * contiguous): pairs (m, m + rot_dim / 2), or (2m, 2m + 1) when interleaved:
  *   x' = x c - y s,  y' = y c + x s   (FP32, one rounding to the cache's type).
  * q, k, v and q_out have the cache's type, head_dim contiguous, and token /
- * head strides that are multiples of 8 elements; q_out may be q. head_dim and
- * rot_dim are multiples of 16; rot_dim = 0 appends without rotation; Hq = 0
- * has no queries. lengths is not modified. Replaces, for a paged cache, the
- * rotation and the cache growth of reference src/qwen_int4/model.py:74-88.
+ * head strides that are multiples of 8 elements, q_out's positive; q_out may
+ * be q. head_dim and rot_dim are multiples of 16; rot_dim = 0 appends without
+ * rotation; Hq = 0 has no queries. lengths is not modified. Replaces, for a
+ * paged cache, the rotation and the cache growth of reference
+ * src/qwen_int4/model.py:74-88.
  */
 QI4_API int qi4_rope_paged_append(const qi4_paged_kv* kv, const void* q, int64_t q_token_stride,
                                   int64_t q_head_stride, const void* k, int64_t k_token_stride,

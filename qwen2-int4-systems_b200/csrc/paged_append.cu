@@ -275,8 +275,8 @@ int check_paged_kv(const qi4_paged_kv* kv, const char* what) {
     return QI4_ERR_SHAPE;
   }
   if (!al16(kv->k) || !al16(kv->v) || kv->page_stride % 8 || kv->head_stride % 8 || kv->slot_stride % 8 ||
-      kv->page_stride < 0 || kv->head_stride < 0 || kv->slot_stride < kv->head_dim) {
-    set_error("%s: pages must be 16-byte aligned, with strides that are multiples of 8 elements", what);
+      kv->page_stride < (kv->pages > 1) || kv->head_stride < (kv->kv_heads > 1) || kv->slot_stride < kv->head_dim) {
+    set_error("%s: pages must be 16-byte aligned, with positive strides that are multiples of 8 elements", what);
     return QI4_ERR_ALIGNMENT;
   }
   return QI4_OK;
@@ -323,9 +323,11 @@ extern "C" QI4_API int qi4_rope_paged_append(const qi4_paged_kv* kv, const void*
                              v_token_stride, v_head_stride, out_token_stride, out_head_stride};
   bool ok = al16(q) && al16(k) && al16(v) && al16(q_out) && al16(cos) && al16(sin);
   for (int64_t s : strides) ok = ok && s % 8 == 0 && s >= 0;
+  // Tokens or heads that share their memory can be read, but not written.
+  ok = ok && out_token_stride >= (Hq && T > 1) && out_head_stride >= (Hq > 1);
   if (!ok) {
     set_error("rotary append: q, k, v, q_out, cos and sin must be 16-byte aligned, with token and head strides that "
-              "are multiples of 8 elements");
+              "are multiples of 8 elements, those of q_out positive");
     return QI4_ERR_ALIGNMENT;
   }
   int sms = 0;

@@ -23,3 +23,22 @@ def test_a_prefix_beyond_its_counts_is_refused(b200, pages, length):
     assert lib.qi4_shared_prefix_attention(ctypes.byref(kv), FAKE, 1536, 128, FAKE, 4, 4, 12, FAKE, pages, length, None,
                                            FAKE, 1, 0.1, None, 0, None) == -3
     assert "prefix" in mod.last_error()
+
+
+@pytest.mark.parametrize("change", [dict(page_stride=0), dict(head_stride=0)])
+def test_pages_and_heads_that_share_their_memory_are_refused(b200, change):
+    mod = importlib.import_module(b200.__name__ + "._lib")
+    lib, kv = mod.load(), _kv(mod, **change)
+    assert lib.qi4_paged_attention(ctypes.byref(kv), FAKE, 1536, 128, FAKE, 4, 4, 12, None, FAKE, 1, 0.1, 1, None, 0,
+                                   None) == -4
+    assert lib.qi4_rope_paged_append(ctypes.byref(kv), FAKE, 1536, 128, FAKE, 256, 128, FAKE, 256, 128, FAKE, 1536, 128,
+                                     4, 4, 12, None, FAKE, None, FAKE, FAKE, 64, 128, 0, None) == -4
+
+
+@pytest.mark.parametrize("token_stride,head_stride", [(0, 128), (1536, 0)])
+def test_rotated_queries_that_share_their_memory_are_refused(b200, token_stride, head_stride):
+    mod = importlib.import_module(b200.__name__ + "._lib")
+    lib, kv = mod.load(), _kv(mod)
+    assert lib.qi4_rope_paged_append(ctypes.byref(kv), FAKE, 1536, 128, FAKE, 256, 128, FAKE, 256, 128, FAKE,
+                                     token_stride, head_stride, 4, 4, 12, None, FAKE, None, FAKE, FAKE, 64, 128, 0,
+                                     None) == -4
