@@ -23,6 +23,8 @@ CASES = [
     (SEQS, 40, 1, 128, F16, -0.05, 0),
     (SEQS, 8, 8, 64, BF16, -0.125, 0),
     ([(4, 700), (90, 1500)], 16, 2, 128, F16, -0.1, 0),
+    ([(5, 700), (4, 30)], 12, 2, 128, BF16, -0.1, 0),  # one tile of 30 rows each, in clusters
+    ([(5, 700)] * 90, 12, 2, 128, F16, -0.1, 0),
     ([(4, 90), (2, 300), (9, 40)], 12, 2, 128, BF16, -0.1, 600),
 ]
 
