@@ -67,6 +67,12 @@ def _owners(cu_tokens, t):
     return torch.searchsorted(cu_tokens[1:], t, right=True).clamp_max(cu_tokens.numel() - 2)
 
 
+def _sample(p, generator):
+    """One token of each row of p [batch, vocabulary]: the first of p / (exponential numbers), as torch.multinomial draws
+    it. Rows that are no numbers give some token, not an assertion on the GPU, after which nothing runs there."""
+    return (p / torch.empty_like(p).exponential_(1, generator=generator)).argmax(dim=-1)
+
+
 class PagedDecoder:
     """``batch`` sequences of up to ``max_len`` keys each (a shared prefix not counted) in pages of ``page_size``."""
 
@@ -191,7 +197,8 @@ def speculative_generate(target: PagedDecoder, draft: PagedDecoder, prompts, max
     follows a shared prefix, if ``set_prefix`` was called on both decoders).
     Each step the draft proposes ``drafts`` tokens per sequence; the target
     reads them in one pass, and ``b200_verify_draft`` keeps those that stand
-    and draws the next. Both caches then go back to the tokens that stand.
+    and draws the next. Both caches then go back to the tokens that stand. A
+    token is -1 where the target's probabilities for it are no numbers.
     """
     if temperature <= 0 or drafts < 1 or max_new_tokens < 1:
         raise ValueError("temperature must be positive, with at least one draft and one new token")
@@ -231,7 +238,7 @@ def speculative_generate(target: PagedDecoder, draft: PagedDecoder, prompts, max
         q = torch.empty(B, drafts, vocab, device=dev)
         for i in range(drafts):
             q[:, i] = probs(draft, draft.forward(tokens[:, i:i + 1]))
-            tokens[:, i + 1] = torch.multinomial(q[:, i], 1, generator=generator)[:, 0]
+            tokens[:, i + 1] = _sample(q[:, i], generator)
         draft.forward(tokens[:, drafts:])  # (the last draft's key, for when it stands)
         p = probs(target, target.forward(tokens)).view(B, drafts + 1, vocab)
         u = torch.rand(B, drafts + 1, device=dev, generator=generator)
@@ -239,7 +246,8 @@ def speculative_generate(target: PagedDecoder, draft: PagedDecoder, prompts, max
         # Sequences that have all their tokens stay where they are.
         step = torch.where(open_, accepted + 1, 0)
         out.scatter_(1, torch.where(open_[:, None], made[:, None] + place, out.shape[1] - 1), found)
-        last = torch.where(open_, found.gather(1, accepted.long()[:, None])[:, 0], last)
+        # (-1 where the target's probabilities are no numbers: the sequence goes on from token 0)
+        last = torch.where(open_, found.gather(1, accepted.long()[:, None])[:, 0].clamp_min(0), last)
         made += step
         target.lengths = torch.minimum(start_t + step, end_t).to(torch.int32)
         draft.lengths = torch.minimum(start_d + step, end_d).to(torch.int32)

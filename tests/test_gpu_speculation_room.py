@@ -1,6 +1,7 @@
 """speculative_generate in the smallest caches that it accepts: sequences that are done early outgrow nothing."""
 
 import importlib
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -76,3 +77,24 @@ def test_generation_goes_on_from_what_the_caches_hold(b200, pe, models, cuda_dev
         dec.lengths = dec.lengths - 1
         got = dec.logits(dec.forward(torch.stack([s[-1:] for s in seqs]))).float()
         assert float((got - want).norm() / want.norm()) < 0.05
+
+
+def _broken(model):
+    """The model with a final norm that makes every logit NaN."""
+    top = SimpleNamespace(weight=torch.full_like(model.model.norm.weight, float("nan")))
+    return SimpleNamespace(config=model.config, lm_head=model.lm_head, model=SimpleNamespace(
+        embed_tokens=model.model.embed_tokens, layers=model.model.layers, norm=top))
+
+
+def test_logits_that_are_no_numbers(b200, pe, models, cuda_device):
+    """A draft without probabilities is refused throughout; of a target without them every token is -1."""
+    prompts = [torch.tensor([3, 4, 5]), torch.tensor([6])]
+    for broken in ("draft", "target", "both"):
+        target = pe.PagedDecoder(_broken(models[0]) if broken != "draft" else models[0], 2, 32)
+        draft = pe.PagedDecoder(_broken(models[0]) if broken != "target" else models[0], 2, 32)
+        tokens, stood = pe.speculative_generate(target, draft, prompts, 6, drafts=2)
+        torch.cuda.synchronize()
+        if broken == "draft":
+            assert int(tokens.min()) >= 0 and int(tokens.max()) < 512 and stood == 0
+        else:
+            assert bool((tokens == -1).all())
