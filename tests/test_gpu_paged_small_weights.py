@@ -4,8 +4,6 @@ The scores are exact: `gap` for the first key, whose value is zero, and 0 for al
 first 16 keys of every 128 alone, where the kernel for few rows takes each group of 16 relative to its own maximum).
 """
 
-import math
-
 import pytest
 import torch
 
@@ -63,3 +61,30 @@ def test_small_weights_count(b200, cuda_device, seqs, prefix, D, groups, gap, dt
     err = (got.double() - ref).abs()
     assert bool((err <= bound).all()), f"worst {(err / bound.clamp_min(1e-30)).max():.3f} of the bound"
     assert bool((ref > 0).any())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("seqs,prefix,D,Hq,Hkv", [
+    ([(1, 480)] * 80, 0, 128, 12, 2),
+    ([(1, 300), (4, 700)], 0, 128, 12, 2),
+    ([(1, 1151)] * 64, 0, 128, 12, 2),
+    ([(5, 3000 + 100 * i) for i in range(12)], 0, 64, 16, 4),
+    ([(1, 9000)], 0, 128, 12, 2),
+    ([(1, 40), (2, 90)], 900, 128, 12, 2),
+])
+def test_few_rows_keep_more_of_a_weight_than_the_type_has(b200, cuda_device, seqs, prefix, D, Hq, Hkv, dtype):
+    """Few rows per key: a weight is a value and its remainder, 2^-16 of it lost at most, which is within the 2^-13 of
+    FP32 scores and sums (_paged.check_attention); only the result is rounded to the type."""
+    x = pg.build(seqs, Hq=Hq, Hkv=Hkv, D=D, page=16, dtype=dtype, device=cuda_device, prefix=prefix)
+    how = dict(cu_tokens=x["cu"], max_tokens=x["most"])
+    if prefix:
+        got = b200.b200_shared_prefix_attention(x["q"], x["k"], x["v"], x["prefix_table"], prefix, x["table"],
+                                                x["lengths"], **how)
+    else:
+        got = b200.b200_paged_attention(x["q"], x["k"], x["v"], x["table"], x["lengths"], **how)
+    ref, size = pg.attention64(x)
+    bound = pg.ROUND[dtype] * ref.abs() + (2.0 ** -16 + 2.0 ** -13) * size
+    if dtype == F16:
+        bound += 2.0 ** -24  # (results below FP16's normal numbers)
+    err = (got.double() - ref).abs()
+    assert bool((err <= bound).all()), f"worst {(err / bound).max():.3f} of the bound"
