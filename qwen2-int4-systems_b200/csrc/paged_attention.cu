@@ -19,13 +19,13 @@
 // released afterwards.
 //
 // Measured (device time, BF16, 12 query heads on 2 KV heads of 128 dims): one
-// sequence of 131,002 keys 30 us, 64 sequences of 1151 keys 22.4 us; per
+// sequence of 131,002 keys 30 us, 64 sequences of 1151 keys 22.7 us; per
 // further unit 6 to 7 TB/s, so what bounds them is the 9 to 11 us of a call
 // that do not grow with the keys: the launch, each warp's way to its first unit
 // (boundaries, lengths and page table, one after the other), the warps' sums,
 // the joining launch. Items that leave two CTAs or more for each, of tables that
 // are not long, are a cluster's work, without a joining launch: one sequence of
-// 641 keys 6.3 us, 16 of 450 keys 6.3.
+// 641 keys 6.5 us, 16 of 450 keys 6.7.
 // Sixteen consumer warps in two groups that take the units
 // by turns had 96 registers each and were slower (25.1 us for the 64).
 #include <cooperative_groups.h>
@@ -615,14 +615,15 @@ namespace {
 // no joining launch follows; half as many for mma.sync items that leave two
 // CTAs or more for each (clusters take those). Lengths are on the device: the
 // tables' width is what the host knows. Split and whole, us: 64 sequences of 500
-// keys, 12 query heads on 2 KV heads of 128 dims 15.3 and 12.0; 1 sequence of
-// 250 keys 8.5 and 7.1, of 500 8.4 and 9.9; 16 prompts of 500 tokens 42.5 and
-// 37.1, 1 prompt of 200 16.4 and 13.3, of 500 18.1 and 17.6. More keys are split
-// although even batches would still gain (64 sequences of 1000 keys: 20.7 and
-// 18.0), for the sake of ragged ones, whose longest sequence would be the bound
-// (64 of up to 1000 keys: 13.8 and 17.4; one of 1000 alone 8.6 and 15.8). A
+// keys, 12 query heads on 2 KV heads of 128 dims 15.7 and 12.3; 1 sequence of
+// 250 keys 8.8 and 7.2, of 500 8.8 and 10.1; 16 prompts of 500 tokens 45.8 and
+// 37.8, 1 prompt of 200 16.8 and 13.7, of 500 18.5 and 17.2. More keys are split
+// although even batches would still gain (64 sequences of 1000 keys: 20.9 and
+// 18.1), for the sake of ragged ones, whose longest sequence would be the bound
+// (64 of up to 1000 keys: 15.7 and 18.4; one of 1000 alone 8.9 and 15.9). A
 // shared prefix, few long items of one length, is always split (500 keys under
-// 64 sequences: 23.1 and 27.6).
+// 64 sequences: 22.7 and 27.7). Wider tables cost the same batch the difference:
+// 64 sequences of 500 keys under tables of 8192 take 15.6 us.
 constexpr int kWholeKeys = 512;
 
 // Where no more items of one row tile are in a batch than clusters of 16, 8, 4
@@ -630,12 +631,11 @@ constexpr int kWholeKeys = 512;
 // largest such, if the tables cover at most kWholeKeys for each of its CTAs and
 // kClusterKeys in all: one launch, no pieces in memory. Dealt to all SMs and in
 // clusters, us (12 query heads on 2 KV heads of 128 dims): one sequence of 641
-// keys 8.4 and 6.3, of 4000 8.9 and 8.0; four of 1000 9.0 and 6.3, of 4000 10.6
-// and 10.4; 16 of 450 10.3 and 6.3, of 2000 14.3 and 11.1; 32 of 900 14.0 and
-// 10.4; ragged, 8 of up to 4000 10.7 and 10.6, 32 of up to 1000 10.4 and 9.7.
+// keys 8.7 and 6.6, of 4000 9.2 and 8.3; four of 1000 9.2 and 6.8, of 4000 10.9
+// and 10.8; 16 of 450 10.3 and 6.7, of 2000 14.4 and 11.7; 32 of 900 14.2 and
+// 11.6; ragged, 8 of up to 4000 10.7 and 10.7, 32 of up to 1000 11.7 and 10.6.
 // Clusters of 16 only where the tables cover more than 8 units (one sequence of
-// 1000 keys: 6.1 in a cluster of 8 and 6.7 of 16; of 2000: 6.7 of 16, four of
-// them in clusters of 8 7.5).
+// 1000 keys took 6.1 in a cluster of 8 and 6.7 of 16 when the rule was made).
 constexpr int kClusterKeys = 4096;
 
 template <int D, int NT, bool F16, bool kClusters>
@@ -719,11 +719,12 @@ cudaError_t launch_kernel(int D, bool f16, int nt, const CUtensorMap& k, const C
 // negative): by the rows of a sequence and KV head. Beyond 32 mma.sync would
 // take several tiles and read the keys for each (48 rows over 1000 keys of a
 // shared prefix 30.7 us by mma.sync, 24.4 by tcgen05, both with the suffix's
-// launches of then); with 128 dims its tile of 32 rows does not fit the
-// registers. mma.sync and tcgen05, us, 64 sequences of 2000 keys, 2 KV heads of
-// 128 dims: 24 rows 46.8 and 49.5, 28 rows 84.0 and 49.7, 32 rows 83.8 and 49.0
-// (one sequence of 300 keys: 8.9 and 13.3, 13.0 and 13.3, 13.2 and 13.1); of 64
-// dims: 24 rows 26.6 and 40.3, 32 rows 31.7 and 39.5.
+// launches of then); with 128 dims its tile of 32 rows does not fit the 168
+// registers that a thread of nine warps can have (592 bytes are spilled, 176 of
+// a tile of 24). mma.sync and tcgen05, us, 64 sequences of 2000 keys, 2 KV heads
+// of 128 dims: 24 rows 49.0 and 49.9, 28 rows 88.6 and 50.2, 32 rows 88.6 and
+// 48.6 (one sequence of 300 keys: 9.6 and 13.8, 13.4 and 13.8, 13.5 and 13.4);
+// of 64 dims: 24 rows 28.9 and 39.5, 32 rows 31.9 and 39.2.
 int64_t tc_from(int D) { return D == 128 ? 25 : 33; }
 bool takes_tc(int64_t tokens, int64_t G, int D, float scale) {
   return tokens * G >= tc_from(D) && G <= 128 && scale >= 0.f;
@@ -864,7 +865,8 @@ int attend(const Call& c, const char* what) {
   cudaError_t e = cudaSuccess;
   // One launch: pieces at `at`, the kernel for `tokens` per sequence. The
   // mma.sync tile is the smallest of 8, 16, 24 and 32 rows that holds them (the
-  // 20 rows of each of 24 ragged sequences of up to 6005 keys, 64 dims: 36.6 us in tiles of 24, 44.6 in tiles of 32).
+  // 20 rows of each of 24 ragged sequences of up to 6005 keys, 64 dims: 36.4 us in tiles of 24, 44.6 in tiles of 32
+  // before the look at odd values, 38.1 in tiles of 24 now).
   auto launch = [&](PagedArgs& x, char* at, int64_t tokens) {
     const bool tc = takes_tc(tokens, G, D, c.scale);
     const size_t rows = takes_tc(tokens, G, D, 1.f) ? kTcRows : 32;

@@ -337,8 +337,8 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 // have their odd values cleared before the product, and at the item's end the
 // rows that see them take them up from the pool: a positive weight times an
 // infinity or NaN is it, whatever the weight. Looking costs what these units'
-// batches take longer by: drafts (24 sequences, 20 rows each) 36.5 -> 37.7 us,
-// ragged chunks 112 -> 115, a prompt of 8192 tokens 248 -> 250.
+// batches take longer by: drafts (24 sequences, 20 rows each) 36.4 -> 38.1 us,
+// ragged chunks 112 -> 116, a prompt of 8192 tokens 249 -> 251.
 
 // Bits 15 and 31: that half of w is infinite or NaN.
 template <bool F16>

@@ -34,11 +34,12 @@
 // Tensor memory: scores 2 x 128 columns, sums 2 x D. All waits are bounded.
 //
 // Measured (device time, BF16, 12 query heads on 2 KV heads of 128 dims): a
-// prompt of 8192 tokens 230 us, 900 TFLOP/s; six ragged chunks of up to 2047
-// tokens 111 us. A unit takes some 4000 cycles: the tensor cores are active for
-// 46% of them and the exponentials' pipe as long. Neither alone is the bound
-// (230 us become 198 without the exponentials, 213 with an eighth of the
-// products): it is the chain scores - maximum - weights - product of a tile,
+// prompt of 8192 tokens 251 us in calls back to back, 820 TFLOP/s; six ragged
+// chunks of up to 2047 tokens 116 us. A unit takes some 4000 cycles: the tensor
+// cores are active for 46% of them and the exponentials' pipe as long. Neither
+// alone is the bound (the 230 us of a short burst, at higher clocks, which the
+// figures below go by, become 198 without the exponentials, 213 with an eighth
+// of the products): it is the chain scores - maximum - weights - product of a tile,
 // which one tile alone takes as long for. Slower were: the maximum and the
 // weights of a whole unit at once (288 us; 276 with registers moved from the
 // other warps), 16 softmax warps of half a row each (313), a warp for the
