@@ -158,7 +158,8 @@ class PagedDecoder:
                                                     cu_tokens=cu_tokens, max_tokens=max_tokens)
             return b200_paged_attention(q, kc, vc, self.table, after, cu_tokens=cu_tokens, max_tokens=max_tokens)
 
-        out = self._layers(tokens, append, attend)
+        with torch.cuda.device(self.device):
+            out = self._layers(tokens, append, attend)
         self.lengths = after.to(torch.int32)
         return out
 
@@ -174,7 +175,8 @@ class PagedDecoder:
         def append(q, k, v, kc, vc):
             return b200_rope_paged_append(q, k, v, kc, vc, table, none, self.cos, self.sin, q_out=q)
 
-        out = self._layers(tokens, append, lambda q, kc, vc: b200_paged_attention(q, kc, vc, table, all_))
+        with torch.cuda.device(self.device):
+            out = self._layers(tokens, append, lambda q, kc, vc: b200_paged_attention(q, kc, vc, table, all_))
         self.prefix_len = n
         self.lengths = torch.zeros_like(self.lengths)
         return out
@@ -183,7 +185,8 @@ class PagedDecoder:
     def logits(self, hidden) -> torch.Tensor:
         """Logits [..., vocabulary] (bf16) over the tied embedding."""
         if hidden.numel() // hidden.shape[-1] <= 8:
-            out, _ = b200_lm_head(hidden, self.model.lm_head.weight, return_argmax=False)
+            with torch.cuda.device(self.device):
+                out, _ = b200_lm_head(hidden, self.model.lm_head.weight, return_argmax=False)
             return out.view(*hidden.shape[:-1], -1)
         return hidden @ self.model.lm_head.weight.t()
 
